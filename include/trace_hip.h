@@ -383,6 +383,96 @@ int trace_upsample2x(const float* in, float* out, int B, int H, int W, int C, in
 int trace_layernorm_image(const float* in, const float* gamma, const float* beta, float* out, int B, int n,
                           float eps, void* stream);
 
+/* ---- operators of attention blocks: what a denoiser that attends along the horizon, or over the agents of a scene, runs
+ * between its plain products.  The reference's denoiser is convolutional (tbsim/models/temporal.py:49-142) and has no
+ * counterpart of these; they come as forward / input-gradient pairs as trace_unet_forward / trace_unet_backward_input do,
+ * because clean guidance differentiates the denoiser (tbsim/models/trace.py:630,640-649).
+ * Unlike the rest of this header their tensors may be fp32, bf16 or fp16 (`dtype`), and strided: strides count
+ * elements, the innermost dimension is contiguous.  Sums, softmax statistics and norms are fp32.  No atomics: the same call
+ * gives the same bits. */
+#define TRACE_F32 0
+#define TRACE_BF16 1
+#define TRACE_F16 2
+
+/* Strides of a (batch, token, head, head element) tensor. */
+typedef struct {
+  int64_t batch, token, head;
+} trace_heads;
+
+/* Attention of q (B, Lq, Hq, D) over k, v (B, Lk, Hk, D); heads hq of q share key head hq / (Hq / Hk).
+ * Query i of sequence b sees key j iff  j < key_lengths[b]  and  key_mask[b, j] != 0  and, if causal,
+ * j <= i + query_start[b].  Keys that no length or mask admits are not read into any result, whatever they hold (NaN
+ * included); of keys that only causality hides from a query this holds as long as they are finite. */
+typedef struct {
+  int dtype;
+  int B, Lq, Lk, Hq, Hk, D;           /* Hq % Hk == 0, 1 <= D <= 128 */
+  float scale;                        /* of the scores; > 0 */
+  int causal;
+  const int* query_start;             /* (B) position of query 0 among the keys; NULL: Lk - Lq */
+  const int* key_lengths;             /* (B), taken as 0 .. Lk; NULL: Lk */
+  const uint8_t* key_mask;            /* (B, Lk), rows key_mask_stride apart; NULL: all */
+  int64_t key_mask_stride;
+  trace_heads q, k, v, out;           /* out: of the forward; the backward pass reads it */
+  trace_heads dout, dq, dk, dv;       /* backward only */
+} trace_attention_desc;
+
+/* Workspace bytes of a call (0: none needed); negative: TRACE_E*. */
+int64_t trace_attention_workspace_bytes(const trace_attention_desc* d, int backward);
+/* out = softmax(scale q k^T) v over the visible keys; lse (B, Hq, Lq) fp32 = log of the softmax denominator.  A query
+ * that sees no key gets out = 0 and lse = -inf. */
+int trace_attention(const trace_attention_desc* d, const void* q, const void* k, const void* v, void* out, float* lse,
+                    void* workspace, int64_t workspace_bytes, void* stream);
+/* Gradients w.r.t. q, k and v given dout and the forward's out and lse; the probabilities are recomputed.  Gradients of
+ * shared key heads are summed over their query heads; queries that see nothing and keys that are not seen get zero. */
+int trace_attention_backward(const trace_attention_desc* d, const void* dout, const void* q, const void* k,
+                             const void* v, const void* out, const float* lse, void* dq, void* dk, void* dv,
+                             void* workspace, int64_t workspace_bytes, void* stream);
+
+/* Rotary positions of q (B, L, Hq, D) and k (B, L, Hk, D; Hk == 0: no k) in one launch: the pair (a, b) number p of a head
+ * at position t becomes  scale (a cos w - b sin w, b cos w + a sin w),  w = t freqs[p] (-w if inverse: the gradient's
+ * way), in 64-bit angles.  Pairs are elements (p, p + rot / 2), or (2p, 2p + 1) if interleaved; elements rot .. D - 1 are
+ * copied.  A result may be its input (same strides); it must not overlap one in any other way. */
+typedef struct {
+  int dtype;
+  int B, L, Hq, Hk, D, rot;           /* D <= 1024; rot even, 2 .. D */
+  int interleaved, inverse;
+  float scale;
+  int wide_positions;                 /* positions are int64 (else int32) */
+  int64_t position_batch_stride;      /* positions[b * stride + l]; 0: one row for all */
+  trace_heads q, k, out_q, out_k;
+} trace_rotary_desc;
+int trace_rotary(const trace_rotary_desc* d, const void* q, const void* k, const void* positions, const double* freqs,
+                 void* out_q, void* out_k, void* stream);
+
+/* The norms before and after a block, fused with the block's gate and the residual connection.  Row r of x, y (rows, C):
+ *   u = N(y) * post_weight   (post_weight NULL: u = y)
+ *   h = residual_scale * x + gate * u                       (gate NULL: 1)
+ *   z = N(h) * weight + bias                                (NULL: 1 / 0)
+ * with row g = r / rows_per_cond of gate if gate_per_cond, and of weight and bias if per_cond.
+ * N(t) = (t - mean) / sqrt(var + eps) or t / sqrt(mean t^2 + eps).  x, h have stream_dtype (TRACE_F32, or dtype); y, z have dtype; gate, weights,
+ * bias and their gradients are fp32.  y NULL: h is x itself (z only: the norm before the first block).
+ * h or z may be NULL: not wanted.  Inputs have row strides; results are contiguous and may not overlap inputs. */
+#define TRACE_NORM_RMS 0
+#define TRACE_NORM_LAYER 1
+typedef struct {
+  int dtype, stream_dtype;
+  int rows, C;                        /* C <= 16384 */
+  int rows_per_cond;                  /* rows of a conditioning group */
+  int per_cond, gate_per_cond;        /* weight and bias / gate have a row per group (else one for all) */
+  int kind;
+  float residual_scale, eps;
+  int64_t x_stride, y_stride, dh_stride, dz_stride;
+} trace_norm_desc;
+int trace_residual_norm(const trace_norm_desc* d, const void* x, const void* y, const float* gate,
+                        const float* post_weight, const float* weight, const float* bias, void* h, void* z, void* stream);
+/* Gradients given dh and dz (either may be NULL: zero), recomputed from x and y.  dx (x's type) and, with y, dy are
+ * written; dgate, dpost_weight, dweight, dbias (the shapes of their parameters) may be NULL.  rows > 0. */
+int64_t trace_residual_norm_workspace_bytes(const trace_norm_desc* d);
+int trace_residual_norm_backward(const trace_norm_desc* d, const void* dh, const void* dz, const void* x, const void* y,
+                                 const float* gate, const float* post_weight, const float* weight, void* dx, void* dy,
+                                 float* dgate, float* dpost_weight, float* dweight, float* dbias, void* workspace,
+                                 int64_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -42,6 +42,30 @@ class StepCoefs(C.Structure):
                 ("sqrt_recip_one_minus_alphas_cumprod", C.c_float), ("t", C.c_int)]
 
 
+class AttentionDesc(C.Structure):
+    # four trace_heads per direction, each three strides, flattened
+    _fields_ = ([("dtype", C.c_int), ("B", C.c_int), ("Lq", C.c_int), ("Lk", C.c_int), ("Hq", C.c_int), ("Hk", C.c_int),
+                 ("D", C.c_int), ("scale", C.c_float), ("causal", C.c_int), ("query_start", C.c_void_p),
+                 ("key_lengths", C.c_void_p), ("key_mask", C.c_void_p), ("key_mask_stride", C.c_int64)] +
+                [("%s_%s" % (t, s), C.c_int64) for t in ("q", "k", "v", "out", "dout", "dq", "dk", "dv")
+                 for s in ("batch", "token", "head")])
+
+
+class RotaryDesc(C.Structure):
+    _fields_ = ([("dtype", C.c_int), ("B", C.c_int), ("L", C.c_int), ("Hq", C.c_int), ("Hk", C.c_int), ("D", C.c_int),
+                 ("rot", C.c_int), ("interleaved", C.c_int), ("inverse", C.c_int), ("scale", C.c_float),
+                 ("wide_positions", C.c_int), ("position_batch_stride", C.c_int64)] +
+                [("%s_%s" % (t, s), C.c_int64) for t in ("q", "k", "out_q", "out_k")
+                 for s in ("batch", "token", "head")])
+
+
+class NormDesc(C.Structure):
+    _fields_ = [("dtype", C.c_int), ("stream_dtype", C.c_int), ("rows", C.c_int), ("C", C.c_int),
+                ("rows_per_cond", C.c_int), ("per_cond", C.c_int), ("gate_per_cond", C.c_int), ("kind", C.c_int), ("residual_scale", C.c_float),
+                ("eps", C.c_float), ("x_stride", C.c_int64), ("y_stride", C.c_int64), ("dh_stride", C.c_int64),
+                ("dz_stride", C.c_int64)]
+
+
 _P = C.c_void_p
 _I = C.c_int
 _F = C.c_float
@@ -99,6 +123,14 @@ PROTOTYPES = {
     "trace_maxpool3x3s2": (_I, [_P, _P, _I, _I, _I, _I, _P]),
     "trace_upsample2x": (_I, [_P, _P, _I, _I, _I, _I, _I, _I, _P]),
     "trace_layernorm_image": (_I, [_P, _P, _P, _P, _I, _I, _F, _P]),
+    "trace_attention_workspace_bytes": (_L, [C.POINTER(AttentionDesc), _I]),
+    "trace_attention": (_I, [C.POINTER(AttentionDesc), _P, _P, _P, _P, _P, _P, _L, _P]),
+    "trace_attention_backward": (_I, [C.POINTER(AttentionDesc), _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _L, _P]),
+    "trace_rotary": (_I, [C.POINTER(RotaryDesc), _P, _P, _P, _P, _P, _P, _P]),
+    "trace_residual_norm": (_I, [C.POINTER(NormDesc), _P, _P, _P, _P, _P, _P, _P, _P, _P]),
+    "trace_residual_norm_workspace_bytes": (_L, [C.POINTER(NormDesc)]),
+    "trace_residual_norm_backward": (_I, [C.POINTER(NormDesc), _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _L,
+                                          _P]),
 }
 
 _lib = None

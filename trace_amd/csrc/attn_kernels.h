@@ -1,0 +1,544 @@
+// Attention and its backward pass (gfx950): the kernels behind trace_attention / trace_attention_backward.
+//
+//   S = scale q k^T over the visible pairs,  lse_i = log sum_j exp S_ij,  out_i = sum_j exp(S_ij - lse_i) v_j
+//   P = exp(S - lse),  delta_i = dout_i . out_i,  dS = P (dout v^T - delta)
+//   dq = scale dS k,  dk = scale dS^T q,  dv = P^T dout
+//
+// One pass over the keys with a running maximum and sum; nothing of size Lq x Lk leaves the registers.  Every product is
+// a 32x32 matrix instruction, and its operands are chosen so that no result is ever shuffled between lanes: S is
+// computed transposed (rows = keys, columns = queries), which leaves lane l with query l & 31 and half of the tile's
+// keys -- exactly the second operand of out^T = V^T P^T once the 16 keys of an instruction are taken in the order
+// 8a + 4h + i -> slot 8h + 4a + i (h: lane half).  The first operands V^T, K^T, Q^T, dO^T come from LDS images that are
+// written transposed and with their keys in that order (TileX); operands read along the head come from TileR.
+#pragma once
+#include "layer_types.h"
+
+namespace trace {
+
+struct AttnView {
+  long sb, sl, sh;      // strides in elements: batch, token, head
+};
+
+struct AttnArgs {
+  const void *q, *k, *v, *out_in, *dout;
+  void *out, *dq, *dk, *dv;
+  const float* lse_in;
+  float* lse;                        // (B, Hq, Lq)
+  float* delta;                      // (B, Hq, Lq), written by the dq kernel, read by the dk / dv kernel
+  AttnView vq, vk, vv, vo, vdo, vdq, vdk, vdv;
+  int B, Lq, Lk, Hq, Hk, G, D;       // G = Hq / Hk query heads share a key head
+  float scale, scale_log2;           // scale, scale * log2(e)
+  int causal;
+  const int* query_start;            // (B) or null
+  const int* key_lengths;            // (B) or null
+  const unsigned char* key_mask;     // (B, Lk) or null
+  long mask_stride;
+  int vec;                           // every pointer and stride 16-byte aligned, D % 8 == 0
+  long items;                        // work items of the launch
+};
+
+constexpr float LOG2E = 1.44269504088896340736f, LN2 = 0.693147180559945309417f;
+
+// ---- LDS images of a tile of ROWS tokens x DP head elements -----------------------------------------------------
+// TileR: token-major; the 16 bytes of padding put the 16-byte pieces of 16 consecutive rows on different banks.
+template <typename T, int DP>
+struct TileR {
+  static constexpr int S = DP + 16 / (int)sizeof(T);
+  static __device__ __forceinline__ int frag(int row, int c, int half) { return row * S + c * 16 + half * 8; }
+};
+// TileX: transposed, element (d, token) with the tokens of each group of 16 in slot order.  The group's two blocks of
+// eight are exchanged with those of other groups by the d >> 4 term: rows 16 apart would otherwise meet on the same banks
+// when eight lanes write eight head elements each (rows are padded, so reads along 32 rows do not conflict).
+template <typename T, int ROWS>
+struct TileX {
+  static constexpr int S = ROWS + 16 / (int)sizeof(T);
+  static constexpr int M = ROWS / 8 - 1;
+  static __device__ __forceinline__ int frag(int d, int c, int half) { return d * S + (((c * 2 + half) ^ ((d >> 4) & M)) << 3); }
+  // tokens 4 quad .. 4 quad + 3
+  static __device__ __forceinline__ int quad(int d, int quad) {
+    const int h = quad & 1, a = (quad >> 1) & 1, c = quad >> 2;
+    return d * S + (((c * 2 + h) ^ ((d >> 4) & M)) << 3) + a * 4;
+  }
+};
+
+// A staging unit is 4 tokens x 8 head elements: unit u of a tile covers tokens 4 (u / (DP/8)) .. + 3.
+template <typename T>
+struct Unit {
+  typename Elem<T>::V8 r[4];
+  // p: element (token 0 of the unit, first head element); n: head elements left of D; valid: bit i = token i exists
+  __device__ __forceinline__ void load(const T* p, long sl, int n, unsigned valid, bool vec) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) r[i] = load8<T>(p + i * sl, (valid >> i) & 1 ? n : 0, vec);
+  }
+  template <int DP>
+  __device__ __forceinline__ void put_r(T* tile, int u) const {
+    const int quad = u / (DP / 8), dc = u % (DP / 8);
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      *reinterpret_cast<typename Elem<T>::V8*>(tile + (quad * 4 + i) * TileR<T, DP>::S + dc * 8) = r[i];
+  }
+  template <int DP, int ROWS>
+  __device__ __forceinline__ void put_x(T* tile, int u) const {
+    const int quad = u / (DP / 8), dc = u % (DP / 8);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      typename Elem<T>::V4 t;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) t[i] = r[i][j];
+      *reinterpret_cast<typename Elem<T>::V4*>(tile + TileX<T, ROWS>::quad(dc * 8 + j, quad)) = t;
+    }
+  }
+};
+
+template <typename T>
+__device__ __forceinline__ const typename Elem<T>::V8 frag_at(const T* tile, int at) {
+  return *reinterpret_cast<const typename Elem<T>::V8*>(tile + at);
+}
+
+// Registers 8c .. 8c + 7 of a 32x32 result as the second operand of the next product (16 of its 32 rows).  The only
+// rounding of P and dS: to the inputs' type, to nearest, as the matrix instruction takes no wider operand.
+template <typename T>
+__device__ __forceinline__ typename Elem<T>::V8 as_operand(const f32x16& s, int c) {
+  typename Elem<T>::V8 v;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) v[i] = (T)s[8 * c + i];
+  return v;
+}
+
+// One bit per key of the tile at key0: below the sequence's length and not masked.  The same in every wave.
+__device__ __forceinline__ unsigned long long key_bits(const AttnArgs& a, int b, int key0, int len) {
+  const int key = key0 + (int)(threadIdx.x & 63);
+  bool on = key < len;
+  if (on && a.key_mask) on = a.key_mask[(long)b * a.mask_stride + key] != 0;
+  return __ballot(on);
+}
+
+__device__ __forceinline__ int key_limit(const AttnArgs& a, int b) {
+  if (!a.key_lengths) return a.Lk;
+  const int n = a.key_lengths[b];
+  return n < 0 ? 0 : (n < a.Lk ? n : a.Lk);
+}
+
+// Query i sees key j iff j <= i + start.  Without causality every key is at or before the start.
+__device__ __forceinline__ long causal_start(const AttnArgs& a, int b) {
+  if (!a.causal) return (long)a.Lk;
+  return a.query_start ? (long)a.query_start[b] : (long)a.Lk - a.Lq;
+}
+
+// ---- forward ------------------------------------------------------------------------------------------------------
+// One workgroup = 32 NW queries of one head, one wave = 32 of them; the keys pass in tiles of 64.
+template <typename T, int DP, int NW>
+__global__ __launch_bounds__(NW * 64) void attn_fwd_kernel(AttnArgs a) {
+  typedef typename Elem<T>::V8 V8;
+  constexpr int KT = 64, NT = NW * 64, NC = DP / 16, ND = DP / 32;
+  constexpr int UN = KT / 4 * (DP / 8), UPT = (2 * UN + NT - 1) / NT;
+  extern __shared__ __attribute__((aligned(16))) char lds[];
+  T* const kt = reinterpret_cast<T*>(lds);
+  T* const vx = kt + KT * TileR<T, DP>::S;
+  const long item = xcd_item(a.items);
+  if (item >= a.items) return;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, col = lane & 31, half = lane >> 5;
+  const int tiles = (a.Lq + 32 * NW - 1) / (32 * NW);
+  const int tile = tiles - 1 - (int)(item % tiles);       // causal: the longest first
+  const int hq = (int)((item / tiles) % a.Hq);
+  const int b = (int)(item / tiles / a.Hq);
+  const int hk = hq / a.G;
+  const int i = tile * 32 * NW + wave * 32 + col;         // this lane's query
+  const bool vec = a.vec != 0;
+
+  V8 qf[NC];
+  {
+    const T* p = (const T*)a.q + b * a.vq.sb + hq * a.vq.sh + (long)i * a.vq.sl;
+#pragma unroll
+    for (int c = 0; c < NC; ++c) {
+      const int d = c * 16 + half * 8;
+      qf[c] = load8<T>(p + d, i < a.Lq ? a.D - d : 0, vec);
+    }
+  }
+  const int len = key_limit(a, b);
+  const long start = causal_start(a, b);
+  const int last_row = min(tile * 32 * NW + 32 * NW, a.Lq) - 1;
+  const long seen = last_row + start + 1;                 // keys the last query of the workgroup sees
+  const int end = (int)max(0L, min((long)len, seen));
+  const long sees = (long)i + start;                      // last key this lane's query sees
+
+  const T* kb = (const T*)a.k + b * a.vk.sb + hk * a.vk.sh;
+  const T* vb = (const T*)a.v + b * a.vv.sb + hk * a.vv.sh;
+  Unit<T> un[UPT];
+  auto fetch = [&](int key0, unsigned long long bits) {
+#pragma unroll
+    for (int n = 0; n < UPT; ++n) {
+      const int u = tid + n * NT;
+      const bool is_v = u >= UN;
+      const int w = is_v ? u - UN : u;
+      const int quad = w / (DP / 8), d = w % (DP / 8) * 8;
+      const unsigned ok = u < 2 * UN ? (unsigned)(bits >> (quad * 4)) & 15u : 0u;
+      const long sl = is_v ? a.vv.sl : a.vk.sl;
+      un[n].load((is_v ? vb : kb) + (long)(key0 + quad * 4) * sl + d, sl, a.D - d, ok, vec);
+    }
+  };
+  auto put = [&]() {
+#pragma unroll
+    for (int n = 0; n < UPT; ++n) {
+      const int u = tid + n * NT;
+      if (u < UN) un[n].template put_r<DP>(kt, u);
+      else if (u < 2 * UN) un[n].template put_x<DP, KT>(vx, u - UN);
+    }
+  };
+
+  f32x16 o[ND] = {};
+  float m = -INFINITY, l = 0.f;                            // l: the sum over this lane half's keys
+  unsigned long long bits = key_bits(a, b, 0, end);
+  fetch(0, bits);
+  for (int key0 = 0; key0 < end; key0 += KT) {
+    __syncthreads();
+    put();
+    __syncthreads();
+    const unsigned long long here = bits;
+    if (key0 + KT < end) {
+      bits = key_bits(a, b, key0 + KT, end);
+      fetch(key0 + KT, bits);
+    }
+    if (here == 0ull) continue;
+    f32x16 s[2] = {};
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+      for (int c = 0; c < NC; ++c) s[t] = Elem<T>::mma32(frag_at<T>(kt, TileR<T, DP>::frag(t * 32 + col, c, half)), qf[c], s[t]);
+    if (here != ~0ull || key0 + KT - 1 > sees - col) {     // sees - col: what the wave's first query sees
+      const unsigned long long mine = here >> (4 * half);
+      const long room = sees - key0 - 4 * half;
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          const int key = t * 32 + 8 * (r / 4) + r % 4;
+          if (!((mine >> key) & 1) || key > room) s[t][r] = -INFINITY;
+        }
+    }
+    float top = -INFINITY;
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) top = fmaxf(top, s[t][r]);
+    top = fmaxf(top, __shfl_xor(top, 32, 64));
+    const float mn = fmaxf(m, top * a.scale_log2);
+    const float use = mn == -INFINITY ? 0.f : mn;          // nothing visible yet: every exponential below is 0
+    const float alpha = __builtin_amdgcn_exp2f(m - use);
+    m = mn;
+    float sum = 0.f;
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        s[t][r] = __builtin_amdgcn_exp2f(fmaf(s[t][r], a.scale_log2, -use));
+        sum += s[t][r];
+      }
+    l = fmaf(l, alpha, sum);
+    if (__any(alpha != 1.f)) {
+#pragma unroll
+      for (int dt = 0; dt < ND; ++dt)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) o[dt][r] *= alpha;
+    }
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        const V8 p = as_operand<T>(s[t], c);
+#pragma unroll
+        for (int dt = 0; dt < ND; ++dt)
+          o[dt] = Elem<T>::mma32(frag_at<T>(vx, TileX<T, KT>::frag(dt * 32 + col, t * 2 + c, half)), p, o[dt]);
+      }
+  }
+  l += __shfl_xor(l, 32, 64);
+  if (i >= a.Lq) return;
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+  T* op = (T*)a.out + b * a.vo.sb + hq * a.vo.sh + (long)i * a.vo.sl;
+#pragma unroll
+  for (int dt = 0; dt < ND; ++dt)
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      const int d = dt * 32 + g * 8 + half * 4;
+      const f32v4 w = {o[dt][4 * g] * inv, o[dt][4 * g + 1] * inv, o[dt][4 * g + 2] * inv, o[dt][4 * g + 3] * inv};
+      if (d < a.D) store4<T>(op + d, w, a.D - d, vec);
+    }
+  if (half == 0) a.lse[((long)b * a.Hq + hq) * a.Lq + i] = l == 0.f ? -INFINITY : (m + log2f(l)) * LN2;
+}
+
+// ---- backward: dq (and delta) ---------------------------------------------------------------------------------------
+// One workgroup = 32 NW queries of one head, keys in tiles of KT: S^T and dP^T = V dO^T share the layout of the forward,
+// dq^T += K^T dS^T.  delta = dout . out is formed here first and left for the dk / dv kernel.
+template <typename T, int DP, int NW>
+__global__ __launch_bounds__(NW * 64) void attn_dq_kernel(AttnArgs a) {
+  typedef typename Elem<T>::V8 V8;
+  constexpr int KT = 64, NT = NW * 64, NC = DP / 16, ND = DP / 32;
+  constexpr int UN = KT / 4 * (DP / 8), UPT = (2 * UN + NT - 1) / NT;
+  extern __shared__ __attribute__((aligned(16))) char lds[];
+  T* const kt = reinterpret_cast<T*>(lds);
+  T* const vt = kt + KT * TileR<T, DP>::S;
+  T* const kx = vt + KT * TileR<T, DP>::S;
+  const long item = xcd_item(a.items);
+  if (item >= a.items) return;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, col = lane & 31, half = lane >> 5;
+  const int tiles = (a.Lq + 32 * NW - 1) / (32 * NW);
+  const int tile = tiles - 1 - (int)(item % tiles);
+  const int hq = (int)((item / tiles) % a.Hq);
+  const int b = (int)(item / tiles / a.Hq);
+  const int hk = hq / a.G;
+  const int i = tile * 32 * NW + wave * 32 + col;
+  const bool vec = a.vec != 0;
+  const long row = ((long)b * a.Hq + hq) * a.Lq + i;
+
+  const float lse = i < a.Lq ? a.lse_in[row] : -INFINITY;
+  const bool live = lse != -INFINITY;                     // a row that sees nothing has no gradient, whatever it holds
+  const float lse2 = live ? lse * LOG2E : INFINITY;
+  V8 qf[NC], gf[NC];
+  float delta = 0.f;
+#pragma unroll
+  for (int c = 0; c < NC; ++c) {
+    const int d = c * 16 + half * 8, n = live ? a.D - d : 0;
+    qf[c] = load8<T>((const T*)a.q + b * a.vq.sb + hq * a.vq.sh + (long)i * a.vq.sl + d, n, vec);
+    gf[c] = load8<T>((const T*)a.dout + b * a.vdo.sb + hq * a.vdo.sh + (long)i * a.vdo.sl + d, n, vec);
+    const V8 of = load8<T>((const T*)a.out_in + b * a.vo.sb + hq * a.vo.sh + (long)i * a.vo.sl + d, n, vec);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) delta = fmaf((float)gf[c][j], (float)of[j], delta);
+  }
+  delta += __shfl_xor(delta, 32, 64);
+  if (half == 0 && i < a.Lq) a.delta[row] = delta;
+
+  const int len = key_limit(a, b);
+  const long start = causal_start(a, b);
+  const int last_row = min(tile * 32 * NW + 32 * NW, a.Lq) - 1;
+  const int end = (int)max(0L, min((long)len, last_row + start + 1));
+  const long sees = (long)i + start;
+  const T* kb = (const T*)a.k + b * a.vk.sb + hk * a.vk.sh;
+  const T* vb = (const T*)a.v + b * a.vv.sb + hk * a.vv.sh;
+  Unit<T> un[UPT];
+  auto fetch = [&](int key0, unsigned long long bits) {
+#pragma unroll
+    for (int n = 0; n < UPT; ++n) {
+      const int u = tid + n * NT;
+      const bool is_v = u >= UN;
+      const int w = is_v ? u - UN : u;
+      const int quad = w / (DP / 8), d = w % (DP / 8) * 8;
+      const unsigned ok = u < 2 * UN ? (unsigned)(bits >> (quad * 4)) & 15u : 0u;
+      const long sl = is_v ? a.vv.sl : a.vk.sl;
+      un[n].load((is_v ? vb : kb) + (long)(key0 + quad * 4) * sl + d, sl, a.D - d, ok, vec);
+    }
+  };
+  auto put = [&]() {
+#pragma unroll
+    for (int n = 0; n < UPT; ++n) {
+      const int u = tid + n * NT;
+      if (u < UN) {
+        un[n].template put_r<DP>(kt, u);
+        un[n].template put_x<DP, KT>(kx, u);
+      } else if (u < 2 * UN) {
+        un[n].template put_r<DP>(vt, u - UN);
+      }
+    }
+  };
+  f32x16 acc[ND] = {};
+  unsigned long long bits = key_bits(a, b, 0, end);
+  fetch(0, bits);
+  for (int key0 = 0; key0 < end; key0 += KT) {
+    __syncthreads();
+    put();
+    __syncthreads();
+    const unsigned long long here = bits;
+    if (key0 + KT < end) {
+      bits = key_bits(a, b, key0 + KT, end);
+      fetch(key0 + KT, bits);
+    }
+    if (here == 0ull) continue;
+    const bool partial = here != ~0ull || key0 + KT - 1 > sees - col;
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      f32x16 s = {}, dp = {};
+#pragma unroll
+      for (int c = 0; c < NC; ++c) s = Elem<T>::mma32(frag_at<T>(kt, TileR<T, DP>::frag(t * 32 + col, c, half)), qf[c], s);
+#pragma unroll
+      for (int c = 0; c < NC; ++c) dp = Elem<T>::mma32(frag_at<T>(vt, TileR<T, DP>::frag(t * 32 + col, c, half)), gf[c], dp);
+#pragma unroll
+      for (int r = 0; r < 16; ++r) s[r] = __builtin_amdgcn_exp2f(fmaf(s[r], a.scale_log2, -lse2)) * (dp[r] - delta);
+      if (partial) {
+        const unsigned long long mine = here >> (4 * half);
+        const long room = sees - key0 - 4 * half;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          const int key = t * 32 + 8 * (r / 4) + r % 4;
+          if (!((mine >> key) & 1) || key > room) s[r] = 0.f;
+        }
+      }
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        const V8 ds = as_operand<T>(s, c);
+#pragma unroll
+        for (int dt = 0; dt < ND; ++dt)
+          acc[dt] = Elem<T>::mma32(frag_at<T>(kx, TileX<T, KT>::frag(dt * 32 + col, t * 2 + c, half)), ds, acc[dt]);
+      }
+    }
+  }
+  if (i >= a.Lq) return;
+  T* p = (T*)a.dq + b * a.vdq.sb + hq * a.vdq.sh + (long)i * a.vdq.sl;
+#pragma unroll
+  for (int dt = 0; dt < ND; ++dt)
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      const int d = dt * 32 + g * 8 + half * 4;
+      const f32v4 w = {acc[dt][4 * g] * a.scale, acc[dt][4 * g + 1] * a.scale, acc[dt][4 * g + 2] * a.scale,
+                       acc[dt][4 * g + 3] * a.scale};
+      if (d < a.D) store4<T>(p + d, w, a.D - d, vec);
+    }
+}
+
+// ---- backward: dk, dv ------------------------------------------------------------------------------------------------
+// One workgroup = 32 NW keys of one key head, one wave = 32 of them; the queries of every head that shares it pass in
+// tiles of 32.  S and dP = dO V^T here have queries as rows: dv^T += dO^T P, dk^T += Q^T dS.  The sums over heads
+// and queries stay in one accumulator in a fixed order: no atomics, the same bits every time.
+template <typename T, int DP, int NW>
+__global__ __launch_bounds__(NW * 64) void attn_dkv_kernel(AttnArgs a) {
+  typedef typename Elem<T>::V8 V8;
+  constexpr int QT = 32, NT = NW * 64, NC = DP / 16, ND = DP / 32;
+  constexpr int UN = QT / 4 * (DP / 8), UPT = (2 * UN + NT - 1) / NT;
+  extern __shared__ __attribute__((aligned(16))) char lds[];
+  T* const qt = reinterpret_cast<T*>(lds);
+  T* const gt = qt + QT * TileR<T, DP>::S;
+  T* const qx = gt + QT * TileR<T, DP>::S;
+  T* const gx = qx + DP * TileX<T, QT>::S;
+  float* const lse2s = reinterpret_cast<float*>(gx + DP * TileX<T, QT>::S);
+  float* const deltas = lse2s + QT;
+  const long item = xcd_item(a.items);
+  if (item >= a.items) return;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, col = lane & 31, half = lane >> 5;
+  const int tiles = (a.Lk + 32 * NW - 1) / (32 * NW);
+  const int tile = (int)(item % tiles);                   // causal: the first keys are seen by the most queries
+  const int hk = (int)((item / tiles) % a.Hk);
+  const int b = (int)(item / tiles / a.Hk);
+  const int key0 = tile * 32 * NW;
+  const int j = key0 + wave * 32 + col;                   // this lane's key
+  const bool vec = a.vec != 0;
+  const int len = key_limit(a, b);
+  const long start = causal_start(a, b);
+  const bool on = j < len && (!a.key_mask || a.key_mask[(long)b * a.mask_stride + j] != 0);
+  V8 kf[NC], vf[NC];
+#pragma unroll
+  for (int c = 0; c < NC; ++c) {
+    const int d = c * 16 + half * 8, n = on ? a.D - d : 0;
+    kf[c] = load8<T>((const T*)a.k + b * a.vk.sb + hk * a.vk.sh + (long)j * a.vk.sl + d, n, vec);
+    vf[c] = load8<T>((const T*)a.v + b * a.vv.sb + hk * a.vv.sh + (long)j * a.vv.sl + d, n, vec);
+  }
+  const int first = (int)max(0L, min((long)a.Lq, (long)key0 - start)) / QT * QT;      // queries before see none of these keys
+  const int per_head = first < a.Lq && key0 < len ? (a.Lq - first + QT - 1) / QT : 0;
+  const int total = per_head * a.G;
+  f32x16 dk[ND] = {}, dv[ND] = {};
+  Unit<T> un[UPT];
+  float row_lse = 0.f, row_delta = 0.f;
+  auto fetch = [&](int n_tile) {
+    const int hq = hk * a.G + n_tile / per_head;
+    const int q0 = first + n_tile % per_head * QT;
+    const float* lse = a.lse_in + ((long)b * a.Hq + hq) * a.Lq;
+#pragma unroll
+    for (int n = 0; n < UPT; ++n) {
+      const int u = tid + n * NT;
+      const bool is_g = u >= UN;
+      const int w = is_g ? u - UN : u;
+      const int quad = w / (DP / 8), d = w % (DP / 8) * 8;
+      unsigned ok = 0;                                    // rows that see nothing count as absent, whatever they hold
+      if (u < 2 * UN) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int r = q0 + quad * 4 + e;
+          if (r < a.Lq && lse[r] != -INFINITY) ok |= 1u << e;
+        }
+      }
+      const AttnView& v = is_g ? a.vdo : a.vq;
+      un[n].load((const T*)(is_g ? a.dout : a.q) + b * v.sb + hq * v.sh + (long)(q0 + quad * 4) * v.sl + d, v.sl,
+                 a.D - d, ok, vec);
+    }
+    if (tid < QT) {
+      const int r = q0 + tid;
+      const float x = r < a.Lq ? lse[r] : -INFINITY;
+      row_lse = x == -INFINITY ? INFINITY : x * LOG2E;
+      row_delta = x == -INFINITY ? 0.f : a.delta[((long)b * a.Hq + hq) * a.Lq + r];
+    }
+  };
+  auto put = [&]() {
+#pragma unroll
+    for (int n = 0; n < UPT; ++n) {
+      const int u = tid + n * NT;
+      if (u < UN) {
+        un[n].template put_r<DP>(qt, u);
+        un[n].template put_x<DP, QT>(qx, u);
+      } else if (u < 2 * UN) {
+        un[n].template put_r<DP>(gt, u - UN);
+        un[n].template put_x<DP, QT>(gx, u - UN);
+      }
+    }
+    if (tid < QT) {
+      lse2s[tid] = row_lse;
+      deltas[tid] = row_delta;
+    }
+  };
+  if (total > 0) fetch(0);
+  for (int n_tile = 0; n_tile < total; ++n_tile) {
+    __syncthreads();
+    put();
+    __syncthreads();
+    const int q0 = first + n_tile % per_head * QT;
+    if (n_tile + 1 < total) fetch(n_tile + 1);
+    if ((long)key0 + wave * 32 > q0 + QT - 1 + start) continue;       // none of the wave's keys is seen
+    const bool partial = (long)key0 + wave * 32 + 31 > q0 + start || !__all(on);
+    f32x16 s = {}, dp = {};
+#pragma unroll
+    for (int c = 0; c < NC; ++c) s = Elem<T>::mma32(frag_at<T>(qt, TileR<T, DP>::frag(col, c, half)), kf[c], s);
+#pragma unroll
+    for (int c = 0; c < NC; ++c) dp = Elem<T>::mma32(frag_at<T>(gt, TileR<T, DP>::frag(col, c, half)), vf[c], dp);
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      const f32v4 ls = *reinterpret_cast<const f32v4*>(lse2s + 8 * g + 4 * half);
+      const f32v4 de = *reinterpret_cast<const f32v4*>(deltas + 8 * g + 4 * half);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int r = 4 * g + e;
+        float p = __builtin_amdgcn_exp2f(fmaf(s[r], a.scale_log2, -ls[e]));
+        float ds = p * (dp[r] - de[e]);
+        if (partial && (!on || (long)j > (long)q0 + 8 * g + 4 * half + e + start)) p = ds = 0.f;
+        s[r] = p;
+        dp[r] = ds;
+      }
+    }
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+      const V8 p = as_operand<T>(s, c);
+#pragma unroll
+      for (int dt = 0; dt < ND; ++dt)
+        dv[dt] = Elem<T>::mma32(frag_at<T>(gx, TileX<T, QT>::frag(dt * 32 + col, c, half)), p, dv[dt]);
+    }
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+      const V8 ds = as_operand<T>(dp, c);
+#pragma unroll
+      for (int dt = 0; dt < ND; ++dt)
+        dk[dt] = Elem<T>::mma32(frag_at<T>(qx, TileX<T, QT>::frag(dt * 32 + col, c, half)), ds, dk[dt]);
+    }
+  }
+  if (j >= a.Lk) return;
+  T* pk = (T*)a.dk + b * a.vdk.sb + hk * a.vdk.sh + (long)j * a.vdk.sl;
+  T* pv = (T*)a.dv + b * a.vdv.sb + hk * a.vdv.sh + (long)j * a.vdv.sl;
+#pragma unroll
+  for (int dt = 0; dt < ND; ++dt)
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      const int d = dt * 32 + g * 8 + half * 4;
+      if (d >= a.D) continue;
+      const f32v4 w = {dk[dt][4 * g] * a.scale, dk[dt][4 * g + 1] * a.scale, dk[dt][4 * g + 2] * a.scale,
+                       dk[dt][4 * g + 3] * a.scale};
+      const f32v4 x = {dv[dt][4 * g], dv[dt][4 * g + 1], dv[dt][4 * g + 2], dv[dt][4 * g + 3]};
+      store4<T>(pk + d, w, a.D - d, vec);
+      store4<T>(pv + d, x, a.D - d, vec);
+    }
+}
+
+}  // namespace trace

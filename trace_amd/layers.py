@@ -1,0 +1,317 @@
+"""Operators of attention blocks on the library's kernels (include/trace_hip.h): attention, rotary positions, and the
+norms before and after a block fused with its gate and the residual connection -- what a denoiser that attends along the
+horizon, or over the agents of a scene, runs between its plain products.
+
+Each comes as a forward and an explicit gradient, as the sampler's own steps do (clean guidance differentiates the denoiser,
+tbsim/models/trace.py:630,640-649); nothing is recorded for autograd, and a tensor that asks for it is refused.
+Tensors are fp32, bf16 or fp16 on one GPU.  Calls only enqueue, on the current stream of that GPU; results and workspaces come
+from torch's allocator, so a call can be captured into a graph.  The same call gives the same bits.
+"""
+import ctypes as C
+import math
+
+import torch
+
+from . import _cabi
+
+_DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+_NORMS = {"rms": 0, "layer": 1}
+
+
+def _need(ok, text, *args):
+    if not ok:
+        raise ValueError(text % args if args else text)
+
+
+def _check(name, t, like=None, dtype=None, shape=None, dims=None):
+    """A tensor that a kernel can take: its type, device and shape, the innermost dimension contiguous."""
+    _need(isinstance(t, torch.Tensor), "%s must be a tensor", name)
+    _need(not (t.requires_grad and torch.is_grad_enabled()),
+          "%s requires grad: these operators record nothing for autograd; call them under torch.no_grad() and use their "
+          "backward functions", name)
+    if dtype is None:
+        _need(t.dtype in _DTYPES, "%s has type %s (float32, bfloat16 or float16)", name, t.dtype)
+    else:
+        _need(t.dtype == dtype, "%s has type %s, expected %s", name, t.dtype, dtype)
+    _need(like is None or t.device == like.device, "%s is on %s, expected %s", name, t.device,
+          like.device if like is not None else None)
+    if shape is not None:
+        _need(tuple(t.shape) == tuple(shape), "%s has shape %s, expected %s", name, tuple(t.shape), tuple(shape))
+    if dims is not None:
+        _need(t.dim() == dims, "%s has %d dimensions, expected %d", name, t.dim(), dims)
+    _need(t.dim() == 0 or t.shape[-1] <= 1 or t.stride(-1) == 1, "the last dimension of %s must be contiguous", name)
+
+
+def _gpu(t):
+    if t.device.type != "cuda":
+        raise _cabi.TraceHipError("the attention-block operators need GPU tensors (got %s); there is no CPU fallback"
+                                  % t.device)
+
+
+def _enqueue(what, device, *args):
+    """The C call `what` on the device's current stream, with the device current."""
+    fn = getattr(_cabi.lib(), what)
+    if device.index == torch.cuda.current_device():
+        rc = fn(*args, torch.cuda.current_stream(device).cuda_stream)
+    else:
+        with torch.cuda.device(device):
+            rc = fn(*args, torch.cuda.current_stream(device).cuda_stream)
+    _cabi.check(rc, what)
+
+
+def _at(t):
+    return None if t is None else t.data_ptr()
+
+
+# ------------------------------------------------------------------------------------------ attention ----
+
+def _attention_desc(q, k, v, causal, query_start, key_lengths, key_mask, scale, rest):
+    _check("q", q, dims=4)
+    _check("k", k, like=q, dtype=q.dtype, dims=4)
+    B, Lq, Hq, D = q.shape
+    Lk, Hk = k.shape[1], k.shape[2]
+    _need(1 <= D <= 128, "head dimension %d unsupported (1..128)", D)
+    _need(tuple(k.shape) == (B, Lk, Hk, D), "k has shape %s, q %s", tuple(k.shape), tuple(q.shape))
+    _check("v", v, like=q, dtype=q.dtype, shape=k.shape)
+    _need(Hk >= 1 and Hq >= 1 and Hq % Hk == 0, "%d query heads cannot share %d key heads", Hq, Hk)
+    _need(max(Lq, Lk) <= 1 << 30, "more than 2^30 tokens")
+    scale = D ** -0.5 if scale is None else float(scale)
+    _need(math.isfinite(scale) and scale > 0, "scale %g must be positive and finite", scale)
+    _need(query_start is None or causal, "query_start has a meaning for causal attention only")
+    for name, t in (("query_start", query_start), ("key_lengths", key_lengths)):
+        if t is not None:
+            _check(name, t, like=q, dtype=torch.int32, shape=(B,))
+    if key_mask is not None:
+        _check("key_mask", key_mask, like=q, dtype=torch.bool, shape=(B, Lk))
+    strides = []
+    for t in (q, k, v) + rest:
+        strides += t.stride()[:3]
+    return _cabi.AttentionDesc(_DTYPES[q.dtype], B, Lq, Lk, Hq, Hk, D, scale, 1 if causal else 0, _at(query_start),
+                               _at(key_lengths), _at(key_mask), 0 if key_mask is None else key_mask.stride(0), *strides)
+
+
+def _workspace(desc, backward, device):
+    n = _cabi.lib().trace_attention_workspace_bytes(C.byref(desc), backward)
+    if n < 0:
+        _cabi.check(int(n), "trace_attention_workspace_bytes")
+    return (torch.empty(n, dtype=torch.uint8, device=device), n) if n else (None, 0)
+
+
+def attention(q, k, v, causal=False, query_start=None, key_lengths=None, key_mask=None, scale=None):
+    """softmax(scale q k^T) v over the visible keys.
+
+    q (B, Lq, Hq, D), k and v (B, Lk, Hk, D): Hq / Hk consecutive query heads share a key head; D <= 128; any strides with
+    the head elements contiguous (windows of one projection's output, say).  scale: D ** -0.5 if None.
+    Query i sees key j iff j < key_lengths[b] (int32), key_mask[b, j] (bool) and, if causal, j <= i + query_start[b]
+    (int32; None: the last query is at the last key, Lk - Lq).  For one new token a sequence on a cache: Lq = 1 and
+    key_lengths.  Keys that no length or mask admits may hold anything, NaN included; keys that only causality hides
+    from some queries have to be finite.
+
+    Returns out (B, Lq, Hq, D) and lse (B, Hq, Lq) fp32, the log of the softmax's denominator: what attention_backward
+    needs.  A query that sees no key gets 0 and -inf."""
+    desc = _attention_desc(q, k, v, causal, query_start, key_lengths, key_mask, scale, ())
+    _gpu(q)
+    B, Lq, Hq, D = q.shape
+    out = torch.empty(B, Lq, Hq, D, dtype=q.dtype, device=q.device)
+    lse = torch.empty(B, Hq, Lq, dtype=torch.float32, device=q.device)
+    desc.out_batch, desc.out_token, desc.out_head = Lq * Hq * D, Hq * D, D
+    ws, n = _workspace(desc, 0, q.device)
+    _enqueue("trace_attention", q.device, C.byref(desc), q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(),
+             lse.data_ptr(), _at(ws), n)
+    return out, lse
+
+
+def attention_backward(dout, q, k, v, out, lse, causal=False, query_start=None, key_lengths=None, key_mask=None,
+                       scale=None):
+    """Gradients (dq, dk, dv) of attention() given dout, its inputs and its results; the probabilities are recomputed.
+    Gradients of shared key heads are summed over their query heads.  Queries that see no key and keys that no query sees get
+    zero, whatever they (and dout) hold there."""
+    _check("q", q, dims=4)
+    _check("dout", dout, like=q, dtype=q.dtype, shape=q.shape)
+    _check("out", out, like=q, dtype=q.dtype, shape=q.shape)
+    _check("lse", lse, like=q, dtype=torch.float32, shape=(q.shape[0], q.shape[2], q.shape[1]))
+    _need(lse.is_contiguous(), "lse must be contiguous")
+    desc = _attention_desc(q, k, v, causal, query_start, key_lengths, key_mask, scale, (out, dout))
+    _gpu(q)
+    dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v))
+    desc.dq_batch, desc.dq_token, desc.dq_head = dq.stride()[:3]
+    desc.dk_batch, desc.dk_token, desc.dk_head = dk.stride()[:3]
+    desc.dv_batch, desc.dv_token, desc.dv_head = dv.stride()[:3]
+    ws, n = _workspace(desc, 1, q.device)
+    _enqueue("trace_attention_backward", q.device, C.byref(desc), dout.data_ptr(), q.data_ptr(), k.data_ptr(),
+             v.data_ptr(), out.data_ptr(), lse.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), _at(ws), n)
+    return dq, dk, dv
+
+
+# --------------------------------------------------------------------------------------------- rotary ----
+
+def rotary_frequencies(rot, base=10000.0, scaling="none", factor=1.0, trained_length=None, turns_kept=32.0,
+                       turns_stretched=1.0, device="cuda"):
+    """Angles a position, for rotary(): (freqs (rot / 2) float64 on `device`, scale).  Pair p turns by
+    base ** (-2 p / rot) a position.  For contexts `factor` times the trained length:
+      "linear"    every angle divided by the factor
+      "base"      the base raised by factor ** (rot / (rot - 2)): the slowest pair is stretched by the factor, the fastest not
+      "by_turns"  pairs that make at least turns_kept turns over trained_length stay, those below turns_stretched are
+                  divided by the factor, a linear ramp in between; scale = 1 + ln(factor) / 10 sharpens the scores"""
+    _need(isinstance(rot, int) and rot >= 2 and rot % 2 == 0, "rot %r must be even and positive", rot)
+    _need(scaling in ("none", "linear", "base", "by_turns"), "unknown scaling %r", scaling)
+    _need(base > 1 and factor >= 1, "base %g must be above 1 and factor %g at least 1", base, factor)
+    _need(scaling != "base" or rot > 2, "scaling by the base needs two pairs")
+    if scaling == "base":
+        base = base * factor ** (rot / (rot - 2))
+    f = float(base) ** (-2 * torch.arange(rot // 2, dtype=torch.float64) / rot)
+    scale = 1.0
+    if scaling == "linear":
+        f = f / factor
+    elif scaling == "by_turns":
+        _need(trained_length is not None and trained_length >= 1, "scaling by turns needs the trained length")
+        _need(turns_kept > turns_stretched, "turns_kept %g must be above turns_stretched %g", turns_kept, turns_stretched)
+        ramp = ((trained_length * f / (2 * math.pi) - turns_stretched) / (turns_kept - turns_stretched)).clamp(0, 1)
+        f = f * ramp + f / factor * (1 - ramp)
+        scale = 1 + 0.1 * math.log(factor)
+    return f.to(device), scale
+
+
+def rotary(q, positions, freqs, k=None, interleaved=False, scale=1.0, inverse=False, inplace=False):
+    """Rotates the first 2 len(freqs) elements of every head of q (B, L, Hq, D), and of k (B, L, Hk, D), by their
+    positions: pair (a, b) number p at position t becomes scale (a cos w - b sin w, b cos w + a sin w), w = t freqs[p],
+    angles in 64 bits.  Pairs are the two halves' elements p, or elements 2p, 2p + 1 if interleaved.  inverse: -w, which
+    is also the gradient (of the same scale).  positions (L) or (B, L), int32 or int64, of any sign; freqs float64.
+    inplace: the results replace q and k.  Returns the rotated q, or (q, k)."""
+    _check("q", q, dims=4)
+    B, L, Hq, D = q.shape
+    if k is not None:
+        _check("k", k, like=q, dtype=q.dtype, dims=4)
+        _need(k.shape[0] == B and k.shape[1] == L and k.shape[3] == D, "k has shape %s, q %s", tuple(k.shape),
+              tuple(q.shape))
+    _check("freqs", freqs, like=q, dtype=torch.float64, dims=1)
+    rot = 2 * freqs.shape[0]
+    _need(2 <= rot <= D <= 1024, "%d rotated of %d head elements (at most 1024)", rot, D)
+    _need(isinstance(positions, torch.Tensor) and positions.dtype in (torch.int32, torch.int64),
+          "positions must be an int32 or int64 tensor")
+    _check("positions", positions, like=q, dtype=positions.dtype)
+    _need(tuple(positions.shape) in ((L,), (B, L)), "positions have shape %s, expected (%d,) or (%d, %d)",
+          tuple(positions.shape), L, B, L)
+    _need(math.isfinite(scale), "scale is not finite")
+    if inplace:
+        for name, t in (("q", q), ("k", k)):
+            _need(t is None or all(s != 0 or n <= 1 for s, n in zip(t.stride(), t.shape)),
+                  "%s is broadcast: it cannot be rotated in place", name)
+    _gpu(q)
+    oq = q if inplace else torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    ok = k if k is None or inplace else torch.empty(k.shape, dtype=k.dtype, device=k.device)
+    none = (0, 0, 0)
+    desc = _cabi.RotaryDesc(_DTYPES[q.dtype], B, L, Hq, 0 if k is None else k.shape[2], D, rot, 1 if interleaved else 0,
+                            1 if inverse else 0, scale, 1 if positions.dtype == torch.int64 else 0,
+                            positions.stride(0) if positions.dim() == 2 else 0, *q.stride()[:3],
+                            *(none if k is None else k.stride()[:3]), *oq.stride()[:3],
+                            *(none if k is None else ok.stride()[:3]))
+    _enqueue("trace_rotary", q.device, C.byref(desc), q.data_ptr(), _at(k), positions.data_ptr(), freqs.data_ptr(),
+             oq.data_ptr(), _at(ok))
+    return oq if k is None else (oq, ok)
+
+
+# ---------------------------------------------------------------------------------------------- norms ----
+
+def _rows(name, t):
+    """t (..., C) as (rows, C) without a copy."""
+    try:
+        return t.view(-1, t.shape[-1]) if t.shape[-1] else t.new_empty(0, 0)
+    except RuntimeError:
+        raise ValueError("%s: the rows of a tensor with strides %s are not evenly spaced" % (name, t.stride()))
+
+
+def _table(name, t, like, groups, C):
+    """A parameter of (C), (1, C) or a row for each conditioning group: whether it has one for each."""
+    if t is None:
+        return False
+    _check(name, t, like=like, dtype=torch.float32)
+    _need(tuple(t.shape) in ((C,), (1, C), (groups, C)), "%s has shape %s, expected (%d,) or (%d, %d)", name,
+          tuple(t.shape), C, groups, C)
+    _need(t.is_contiguous(), "%s must be contiguous", name)
+    return t.dim() == 2 and groups > 1 and t.shape[0] == groups
+
+
+def _norm_desc(x, y, gate, post_weight, weight, bias, kind, residual_scale, eps, rows_per_cond):
+    _check("x", x)
+    _need(x.dim() >= 1 and 1 <= x.shape[-1] <= 16384, "x has shape %s (1..16384 columns)", tuple(x.shape))
+    C_ = x.shape[-1]
+    xr, yr = _rows("x", x), None
+    if y is not None:
+        _check("y", y, like=x, shape=x.shape)
+        _need(x.dtype in (torch.float32, y.dtype), "x is %s beside a block output of %s (float32, or the same)", x.dtype,
+              y.dtype)
+        yr = _rows("y", y)
+    else:
+        _need(gate is None and post_weight is None, "gate and post_weight belong to a block output y")
+    R = xr.shape[0]
+    _need(R < 1 << 31, "more than 2^31 rows")
+    _need(kind in _NORMS, "unknown norm %r", kind)
+    _need(math.isfinite(eps) and eps >= 0 and math.isfinite(residual_scale),
+          "eps %g and residual_scale %g must be finite, eps not negative", eps, residual_scale)
+    _need(rows_per_cond is None or (isinstance(rows_per_cond, int) and rows_per_cond >= 1),
+          "rows_per_cond %r must be a positive number", rows_per_cond)
+    rpc = min(rows_per_cond or max(R, 1), max(R, 1))
+    groups = -(-R // rpc) if R else 1
+    gate_cond = _table("gate", gate, x, groups, C_)
+    _need(not _table("post_weight", post_weight, x, 1, C_), "post_weight has one row")
+    w_cond, b_cond = _table("weight", weight, x, groups, C_), _table("bias", bias, x, groups, C_)
+    _need(weight is None or bias is None or w_cond == b_cond, "weight and bias must both have a row for each group, or "
+          "neither")
+    out = y if y is not None else x
+    return _cabi.NormDesc(_DTYPES[out.dtype], _DTYPES[x.dtype], R, C_, rpc, 1 if w_cond or b_cond else 0,
+                          1 if gate_cond else 0, _NORMS[kind], residual_scale, eps, xr.stride(0),
+                          0 if y is None else yr.stride(0), 0, 0)
+
+
+def residual_norm(x, y=None, gate=None, post_weight=None, weight=None, bias=None, kind="rms", residual_scale=1.0,
+                  eps=1e-5, rows_per_cond=None, norm=True):
+    """The norm after a block, its gate, the residual connection and the norm before the next block, in one pass:
+      u = N(y) * post_weight  (y itself without post_weight),  h = residual_scale * x + gate * u,  z = N(h) * weight + bias
+    over the rows of x and y (..., C): N is the "rms" or "layer" norm of a row.  Without y (before the first block) h is x;
+    norm=False (after the last) leaves z out.  gate, weight and bias (fp32) are (C), or (groups, C) with a row for each
+    rows_per_cond consecutive rows of x: the scale, shift and gate that a conditioning gives to each trajectory.
+    x, the residual stream, has y's type or fp32.  Returns (h, z); h is x where y is None, z None where norm is False."""
+    desc = _norm_desc(x, y, gate, post_weight, weight, bias, kind, residual_scale, eps, rows_per_cond)
+    _need(norm or y is not None, "nothing to compute: no block output and no norm")
+    _need(norm or (weight is None and bias is None), "weight and bias belong to the norm")
+    _gpu(x)
+    h = x if y is None else torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    z = torch.empty(x.shape, dtype=x.dtype if y is None else y.dtype, device=x.device) if norm else None
+    _enqueue("trace_residual_norm", x.device, C.byref(desc), x.data_ptr(), _at(y), _at(gate), _at(post_weight),
+             _at(weight), _at(bias), None if y is None else h.data_ptr(), _at(z))
+    return h, z
+
+
+def residual_norm_backward(dh, dz, x, y=None, gate=None, post_weight=None, weight=None, bias=None, kind="rms",
+                           residual_scale=1.0, eps=1e-5, rows_per_cond=None):
+    """Gradients of residual_norm() given those of its results (either may be None: zero), recomputed from x and y.
+    Returns a dict of dx, dy, dgate, dpost_weight, dweight and dbias; None for what the call does not have."""
+    desc = _norm_desc(x, y, gate, post_weight, weight, bias, kind, residual_scale, eps, rows_per_cond)
+    out = x if y is None else y
+    _need(dh is not None or dz is not None, "neither dh nor dz")
+    if dh is not None:
+        _check("dh", dh, like=x, dtype=x.dtype, shape=x.shape)
+        desc.dh_stride = _rows("dh", dh).stride(0)
+    if dz is not None:
+        _check("dz", dz, like=x, dtype=out.dtype, shape=x.shape)
+        desc.dz_stride = _rows("dz", dz).stride(0)
+    _gpu(x)
+    new = torch.empty if desc.rows and dz is not None else torch.zeros
+    got = {"dx": torch.empty(x.shape, dtype=x.dtype, device=x.device),
+           "dy": None if y is None else torch.empty(y.shape, dtype=y.dtype, device=x.device)}
+    for name, t, f in (("dgate", gate, torch.empty if desc.rows else torch.zeros),
+                       ("dpost_weight", post_weight, torch.empty if desc.rows else torch.zeros),
+                       ("dweight", weight, new), ("dbias", bias, new)):
+        got[name] = None if t is None else f(t.shape, dtype=torch.float32, device=x.device)
+    if not desc.rows:
+        return got
+    n = _cabi.lib().trace_residual_norm_workspace_bytes(C.byref(desc))
+    if n < 0:
+        _cabi.check(int(n), "trace_residual_norm_workspace_bytes")
+    ws = torch.empty(n, dtype=torch.uint8, device=x.device)
+    _enqueue("trace_residual_norm_backward", x.device, C.byref(desc), _at(dh), _at(dz), x.data_ptr(), _at(y), _at(gate),
+             _at(post_weight), _at(weight), got["dx"].data_ptr(), _at(got["dy"]), _at(got["dgate"]),
+             _at(got["dpost_weight"]), _at(got["dweight"]) if dz is not None else None,
+             _at(got["dbias"]) if dz is not None else None, ws.data_ptr(), n)
+    return got
