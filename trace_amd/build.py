@@ -25,6 +25,9 @@ SOURCES = [
     ("guidance.hip", ["-ffp-contract=off"]),
     ("conv2d.hip", ["-fno-slp-vectorize"]),
     ("attention.hip", ["-fno-slp-vectorize"]),
+    ("attn_f32.hip", ["-fno-slp-vectorize"]),
+    ("attn_bf16.hip", ["-fno-slp-vectorize"]),
+    ("attn_f16.hip", ["-fno-slp-vectorize"]),
     ("norm.hip", ["-fno-slp-vectorize"]),
     ("rotary.hip", ["-fno-slp-vectorize"]),
 ]

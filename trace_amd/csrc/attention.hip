@@ -47,57 +47,35 @@ AttnArgs common_args(const trace_attention_desc& d) {
   return a;
 }
 
-template <typename K>
-int launch(K kernel, unsigned long long* attr, size_t lds, int threads, const AttnArgs& a, hipStream_t st, const char* what) {
-  const long grid = xcd_grid(a.items);
-  TRACE_REQUIRE(grid < 0x7fffffffL, "%s: grid of %ld workgroups", what, grid);
-  if (lds > 64 * 1024) TRACE_CHECK_HIP(ensure_dynamic_lds(attr, reinterpret_cast<const void*>(kernel), (int)lds));
-  hipLaunchKernelGGL(kernel, dim3((unsigned)grid), dim3(threads), lds, st, a);
-  return launch_status(what);
-}
-
-// Waves of a workgroup: as many as the 32-row tiles that one (batch, head) has, up to four -- a sequence of 52 steps
-// keeps two busy.
-int waves_for(int rows) { return rows <= 32 ? 1 : rows <= 64 ? 2 : 4; }
-
-template <typename T, int DP, int NW>
-int fwd(AttnArgs a, hipStream_t st) {
-  static unsigned long long attr = 0;
-  a.items = (long)((a.Lq + 32 * NW - 1) / (32 * NW)) * a.Hq * a.B;
-  const size_t lds = sizeof(T) * (64 * TileR<T, DP>::S + DP * TileX<T, 64>::S);
-  return launch(&attn_fwd_kernel<T, DP, NW>, &attr, lds, NW * 64, a, st, "attn_fwd_kernel");
-}
-
-template <typename T, int DP, int NW>
-int dq(AttnArgs a, hipStream_t st) {
-  static unsigned long long attr = 0;
-  a.items = (long)((a.Lq + 32 * NW - 1) / (32 * NW)) * a.Hq * a.B;
-  const size_t lds = sizeof(T) * (2 * 64 * TileR<T, DP>::S + DP * TileX<T, 64>::S);
-  return launch(&attn_dq_kernel<T, DP, NW>, &attr, lds, NW * 64, a, st, "attn_dq_kernel");
-}
-
-template <typename T, int DP, int NW>
-int dkv(AttnArgs a, hipStream_t st) {
-  static unsigned long long attr = 0;
-  a.items = (long)((a.Lk + 32 * NW - 1) / (32 * NW)) * a.Hk * a.B;
-  const size_t lds = sizeof(T) * 2 * (32 * TileR<T, DP>::S + DP * TileX<T, 32>::S) + 2 * 32 * sizeof(float);
-  return launch(&attn_dkv_kernel<T, DP, NW>, &attr, lds, NW * 64, a, st, "attn_dkv_kernel");
-}
-
-#define TRACE_ATTN_NW(FN, T, DP, W) (W == 1 ? FN<T, DP, 1>(a, st) : W == 2 ? FN<T, DP, 2>(a, st) : FN<T, DP, 4>(a, st))
-#define TRACE_ATTN_PICK(NAME, FN, LEN)                                                                     \
-  template <typename T>                                                                                    \
-  int NAME##_t(const AttnArgs& a, hipStream_t st) {                                                        \
-    const int w = waves_for(LEN);                                                                          \
-    return a.D <= 32 ? TRACE_ATTN_NW(FN, T, 32, w) : a.D <= 64 ? TRACE_ATTN_NW(FN, T, 64, w) : TRACE_ATTN_NW(FN, T, 128, w); \
-  }                                                                                                        \
-  int NAME(int dtype, const AttnArgs& a, hipStream_t st) {                                                 \
-    return dtype == TRACE_F32 ? NAME##_t<float>(a, st) : dtype == TRACE_BF16 ? NAME##_t<__bf16>(a, st)     \
-                                                                             : NAME##_t<_Float16>(a, st);  \
+// The form for few queries.  waves: enough to keep every CU's memory queue full (8 a CU measured best); a range has at
+// least 64 keys.
+struct FewPlan {
+  bool use;
+  int splits;
+  int64_t rows, ml_bytes, bytes;     // bytes of workspace
+};
+FewPlan few_plan(const trace_attention_desc& d) {
+  const int G = d.Hq / d.Hk;
+  const int64_t N = (int64_t)d.Lq * G, tiles = (N + 31) / 32, pairs = (int64_t)d.B * d.Hk;
+  FewPlan p{};
+  p.use = d.Lq <= 16;
+  int64_t splits = (2048 + pairs * tiles - 1) / (pairs * tiles);
+  const int64_t most = (d.Lk + 63) / 64;
+  splits = splits < most ? splits : most;
+  p.splits = (int)(splits < 1 ? 1 : splits < ATTN_MAX_SPLITS ? splits : ATTN_MAX_SPLITS);
+  p.rows = pairs * N;
+  if (p.use && p.splits > 1) {
+    p.ml_bytes = (p.rows * p.splits * 2 * (int64_t)sizeof(float) + 15) / 16 * 16;
+    p.bytes = p.ml_bytes + p.rows * p.splits * (d.D <= 32 ? 32 : d.D <= 64 ? 64 : 128) * (int64_t)sizeof(float);
   }
-TRACE_ATTN_PICK(run_fwd, fwd, a.Lq)
-TRACE_ATTN_PICK(run_dq, dq, a.Lq)
-TRACE_ATTN_PICK(run_dkv, dkv, a.Lk)
+  return p;
+}
+
+int by_type(int dtype, AttnPass pass, const AttnArgs& a, hipStream_t st) {
+  return dtype == TRACE_F32    ? attn_run<float>(pass, a, st)
+         : dtype == TRACE_BF16 ? attn_run<__bf16>(pass, a, st)
+                               : attn_run<_Float16>(pass, a, st);
+}
 
 }  // namespace
 }  // namespace trace
@@ -107,7 +85,8 @@ using namespace trace;
 extern "C" int64_t trace_attention_workspace_bytes(const trace_attention_desc* d, int backward) {
   const int rc = check_desc(d, "trace_attention_workspace_bytes");
   if (rc != TRACE_OK) return rc;
-  return backward ? (int64_t)d->B * d->Hq * d->Lq * (int64_t)sizeof(float) : 0;
+  if (d->B == 0 || d->Lq == 0) return 0;
+  return backward ? (int64_t)d->B * d->Hq * d->Lq * (int64_t)sizeof(float) : few_plan(*d).bytes;
 }
 
 extern "C" int trace_attention(const trace_attention_desc* d, const void* q, const void* k, const void* v, void* out,
@@ -116,8 +95,13 @@ extern "C" int trace_attention(const trace_attention_desc* d, const void* q, con
   if (rc != TRACE_OK) return rc;
   if (d->B == 0 || d->Lq == 0) return TRACE_OK;
   TRACE_REQUIRE(q && out && lse && (d->Lk == 0 || (k && v)), "trace_attention: null argument");
-  (void)workspace;
-  (void)workspace_bytes;
+  const FewPlan plan = few_plan(*d);
+  if (plan.bytes > 0 && (!workspace || workspace_bytes < plan.bytes)) {
+    set_error("trace_attention: workspace too small (%lld bytes, need %lld)", (long long)workspace_bytes,
+              (long long)plan.bytes);
+    return TRACE_ENOMEM;
+  }
+  TRACE_REQUIRE(plan.bytes == 0 || aligned16(workspace), "trace_attention: workspace must be 16-byte aligned");
   AttnArgs a = common_args(*d);
   Check c{*d, d->dtype == TRACE_F32 ? 4 : 2, d->D % 8 == 0};
   a.q = q; a.vq = c.view(d->q, q);
@@ -126,7 +110,14 @@ extern "C" int trace_attention(const trace_attention_desc* d, const void* q, con
   a.out = out; a.vo = c.view(d->out, out);
   a.lse = lse;
   a.vec = c.vec;
-  return run_fwd(d->dtype, a, (hipStream_t)stream);
+  if (plan.use) {
+    a.splits = plan.splits;
+    a.part_ml = static_cast<float*>(workspace);
+    a.part_o = reinterpret_cast<float*>(static_cast<char*>(workspace) + plan.ml_bytes);
+    a.items = (int64_t)d->B * d->Hk * (((int64_t)d->Lq * a.G + 31) / 32) * plan.splits;
+    return by_type(d->dtype, AttnPass::few, a, (hipStream_t)stream);
+  }
+  return by_type(d->dtype, AttnPass::forward, a, (hipStream_t)stream);
 }
 
 extern "C" int trace_attention_backward(const trace_attention_desc* d, const void* dout, const void* q, const void* k,
@@ -157,8 +148,8 @@ extern "C" int trace_attention_backward(const trace_attention_desc* d, const voi
   a.delta = static_cast<float*>(workspace);
   a.vec = c.vec;
   if (d->Lq > 0) {
-    const int r = run_dq(d->dtype, a, (hipStream_t)stream);
+    const int r = by_type(d->dtype, AttnPass::dq, a, (hipStream_t)stream);
     if (r != TRACE_OK) return r;
   }
-  return d->Lk > 0 ? run_dkv(d->dtype, a, (hipStream_t)stream) : TRACE_OK;
+  return d->Lk > 0 ? by_type(d->dtype, AttnPass::dkv, a, (hipStream_t)stream) : TRACE_OK;
 }

@@ -34,8 +34,15 @@ struct AttnArgs {
   const unsigned char* key_mask;     // (B, Lk) or null
   long mask_stride;
   int vec;                           // every pointer and stride 16-byte aligned, D % 8 == 0
+  int splits;                        // ranges of keys (attn_few_kernel)
+  float *part_ml, *part_o;           // their partial results: (rows, splits, 2), (rows, splits, padded D)
   long items;                        // work items of the launch
 };
+constexpr int ATTN_MAX_SPLITS = 256;
+
+enum class AttnPass { forward, few, dq, dkv };
+template <typename T>
+int attn_run(AttnPass pass, const AttnArgs& a, hipStream_t st);
 
 constexpr float LOG2E = 1.44269504088896340736f, LN2 = 0.693147180559945309417f;
 
@@ -264,6 +271,187 @@ __global__ __launch_bounds__(NW * 64) void attn_fwd_kernel(AttnArgs a) {
       if (d < a.D) store4<T>(op + d, w, a.D - d, vec);
     }
   if (half == 0) a.lse[((long)b * a.Hq + hq) * a.Lq + i] = l == 0.f ? -INFINITY : (m + log2f(l)) * LN2;
+}
+
+// ---- forward of few queries over many keys ---------------------------------------------------------------------------
+// The queries of all heads that share a key head are the columns of one tile: column n = i G + g.  A workgroup is one wave
+// with 32 columns and one of `splits` ranges of the sequence's keys, so a cache is read once and by the whole chip however
+// few its queries are; attn_join_kernel joins the ranges.  HBM-bound: per 32 keys a wave has 32 D elements of k (straight to the
+// operand's registers) and of v (transposed through LDS of its own, no barriers) in flight while it works on the last 32.
+template <typename T, int DP>
+__global__ __launch_bounds__(64) void attn_few_kernel(AttnArgs a) {
+  typedef typename Elem<T>::V8 V8;
+  constexpr int KT = 32, NC = DP / 16, ND = DP / 32, UPT = KT / 4 * (DP / 8) / 64 > 0 ? KT / 4 * (DP / 8) / 64 : 1;
+  __shared__ __attribute__((aligned(16))) T vx[DP * TileX<T, KT>::S];
+  const long item = xcd_item(a.items);
+  if (item >= a.items) return;
+  const int lane = threadIdx.x & 63, col = lane & 31, half = lane >> 5;
+  const int N = a.Lq * a.G, tiles = (N + 31) / 32;
+  const int split = (int)(item % a.splits);
+  const int tile = (int)((item / a.splits) % tiles);
+  const long pair = item / a.splits / tiles;
+  const int hk = (int)(pair % a.Hk), b = (int)(pair / a.Hk);
+  const int n = tile * 32 + col;
+  const int i = n / a.G, hq = hk * a.G + n % a.G;
+  const bool vec = a.vec != 0;
+  V8 qf[NC];
+  {
+    const T* p = (const T*)a.q + b * a.vq.sb + hq * a.vq.sh + (long)i * a.vq.sl;
+#pragma unroll
+    for (int c = 0; c < NC; ++c) qf[c] = load8<T>(p + c * 16 + half * 8, n < N ? a.D - c * 16 - half * 8 : 0, vec);
+  }
+  const long start = causal_start(a, b);
+  const long sees = (long)i + start;
+  const int last_i = min(tile * 32 + 31, N - 1) / a.G;
+  const int len = (int)max(0L, min((long)key_limit(a, b), last_i + start + 1));
+  const int each = ((len + a.splits - 1) / a.splits + KT - 1) / KT * KT;
+  const int from = (int)min((long)len, (long)split * each), end = min(len, from + each);
+  const T* kb = (const T*)a.k + b * a.vk.sb + hk * a.vk.sh;
+  const T* vb = (const T*)a.v + b * a.vv.sb + hk * a.vv.sh;
+  V8 kf[NC];
+  Unit<T> un[UPT];
+  auto fetch = [&](int key0, unsigned bits) {
+    const int key = key0 + col;
+    const T* p = kb + (long)key * a.vk.sl;
+    const bool on = (bits >> col) & 1;
+#pragma unroll
+    for (int c = 0; c < NC; ++c) kf[c] = load8<T>(p + c * 16 + half * 8, on ? a.D - c * 16 - half * 8 : 0, vec);
+#pragma unroll
+    for (int m = 0; m < UPT; ++m) {
+      const int u = lane + m * 64, quad = u / (DP / 8), d = u % (DP / 8) * 8;
+      const unsigned ok = quad < KT / 4 ? (bits >> (quad * 4)) & 15u : 0u;
+      un[m].load(vb + (long)(key0 + quad * 4) * a.vv.sl + d, a.vv.sl, a.D - d, ok, vec);
+    }
+  };
+  f32x16 o[ND] = {};
+  float m = -INFINITY, l = 0.f;
+  unsigned bits = (unsigned)key_bits(a, b, from, end);
+  fetch(from, bits);
+  for (int key0 = from; key0 < end; key0 += KT) {
+    const unsigned here = bits;
+    f32x16 s = {};
+#pragma unroll
+    for (int c = 0; c < NC; ++c) s = Elem<T>::mma32(kf[c], qf[c], s);
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");   // the last tile's reads of vx come first
+    __builtin_amdgcn_wave_barrier();
+#pragma unroll
+    for (int e = 0; e < UPT; ++e)
+      if (lane + e * 64 < KT / 4 * (DP / 8)) un[e].template put_x<DP, KT>(vx, lane + e * 64);
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    if (key0 + KT < end) {
+      bits = (unsigned)key_bits(a, b, key0 + KT, end);
+      fetch(key0 + KT, bits);
+    }
+    if (here == 0u) continue;
+    if (here != ~0u || key0 + KT - 1 > start) {              // start: what query 0 sees
+      const unsigned mine = here >> (4 * half);
+      const long room = sees - key0 - 4 * half;
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        const int key = 8 * (r / 4) + r % 4;
+        if (!((mine >> key) & 1) || key > room) s[r] = -INFINITY;
+      }
+    }
+    float top = s[0];
+#pragma unroll
+    for (int r = 1; r < 16; ++r) top = fmaxf(top, s[r]);
+    top = fmaxf(top, __shfl_xor(top, 32, 64));
+    const float mn = fmaxf(m, top * a.scale_log2);
+    const float use = mn == -INFINITY ? 0.f : mn;
+    const float alpha = __builtin_amdgcn_exp2f(m - use);
+    m = mn;
+    float sum = 0.f;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+      s[r] = __builtin_amdgcn_exp2f(fmaf(s[r], a.scale_log2, -use));
+      sum += s[r];
+    }
+    l = fmaf(l, alpha, sum);
+    if (__any(alpha != 1.f)) {
+#pragma unroll
+      for (int dt = 0; dt < ND; ++dt)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) o[dt][r] *= alpha;
+    }
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+      const V8 p = as_operand<T>(s, c);
+#pragma unroll
+      for (int dt = 0; dt < ND; ++dt)
+        o[dt] = Elem<T>::mma32(frag_at<T>(vx, TileX<T, KT>::frag(dt * 32 + col, c, half)), p, o[dt]);
+    }
+  }
+  l += __shfl_xor(l, 32, 64);
+  if (n >= N) return;
+  if (a.splits == 1) {
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    T* op = (T*)a.out + b * a.vo.sb + hq * a.vo.sh + (long)i * a.vo.sl;
+#pragma unroll
+    for (int dt = 0; dt < ND; ++dt)
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        const int d = dt * 32 + g * 8 + half * 4;
+        const f32v4 w = {o[dt][4 * g] * inv, o[dt][4 * g + 1] * inv, o[dt][4 * g + 2] * inv, o[dt][4 * g + 3] * inv};
+        if (d < a.D) store4<T>(op + d, w, a.D - d, vec);
+      }
+    if (half == 0) a.lse[((long)b * a.Hq + hq) * a.Lq + i] = l == 0.f ? -INFINITY : (m + log2f(l)) * LN2;
+    return;
+  }
+  // partial results: maximum and sum of the row's range, and its unnormalised output (not written where nothing was seen)
+  const long row = ((pair * N + n) * a.splits + split);
+  if (half == 0) reinterpret_cast<f32v2*>(a.part_ml)[row] = f32v2{m, l};
+  if (l == 0.f) return;
+  float* op = a.part_o + row * DP;
+#pragma unroll
+  for (int dt = 0; dt < ND; ++dt)
+#pragma unroll
+    for (int g = 0; g < 4; ++g)
+      *reinterpret_cast<f32v4*>(op + dt * 32 + g * 8 + half * 4) =
+          f32v4{o[dt][4 * g], o[dt][4 * g + 1], o[dt][4 * g + 2], o[dt][4 * g + 3]};
+}
+
+// One workgroup joins the `splits` partial results of one query: out = sum_s 2^(m_s - M) o_s / sum_s 2^(m_s - M) l_s.
+// Lane groups of DP take every (256 / DP)-th range.
+template <typename T, int DP>
+__global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a) {
+  constexpr int GR = 256 / DP;
+  __shared__ float weight[ATTN_MAX_SPLITS];
+  __shared__ float sums[256];
+  const long row = blockIdx.x;                             // (b Hk + hk) N + n
+  const int N = a.Lq * a.G, n = (int)(row % N);
+  const long pair = row / N;
+  const int hk = (int)(pair % a.Hk), b = (int)(pair / a.Hk), i = n / a.G, hq = hk * a.G + n % a.G;
+  const f32v2* ml = reinterpret_cast<const f32v2*>(a.part_ml) + row * a.splits;
+  const int tid = threadIdx.x, lane = tid & 63;
+  // every wave finds the maximum and the sum for itself
+  float top = -INFINITY;
+  for (int s = lane; s < a.splits; s += 64) top = fmaxf(top, ml[s][0]);
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o, 64));
+  const float use = top == -INFINITY ? 0.f : top;
+  float l = 0.f;
+  for (int s = lane; s < a.splits; s += 64) {
+    const f32v2 v = ml[s];
+    const float w = v[1] == 0.f ? 0.f : __builtin_amdgcn_exp2f(v[0] - use);
+    l += v[1] == 0.f ? 0.f : w * v[1];
+    if (tid < 64) weight[s] = v[1] == 0.f ? -1.f : w;      // -1: nothing was written there
+  }
+  l = wave_sum(l);
+  __syncthreads();
+  const int d = tid % DP, g = tid / DP;
+  float t = 0.f;
+  for (int s = g; s < a.splits; s += GR) {
+    const float w = weight[s];
+    if (w >= 0.f || w != w) t = fmaf(w, a.part_o[(row * a.splits + s) * DP + d], t);
+  }
+  sums[tid] = t;
+  __syncthreads();
+  if (g > 0 || d >= a.D) return;
+#pragma unroll
+  for (int k = 1; k < GR; ++k) t += sums[k * DP + d];
+  ((T*)a.out)[b * a.vo.sb + hq * a.vo.sh + (long)i * a.vo.sl + d] = (T)(l == 0.f ? 0.f : t / l);
+  if (d == 0) a.lse[((long)b * a.Hq + hq) * a.Lq + i] = l == 0.f ? -INFINITY : (top + log2f(l)) * LN2;
 }
 
 // ---- backward: dq (and delta) ---------------------------------------------------------------------------------------

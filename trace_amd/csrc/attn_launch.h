@@ -1,0 +1,73 @@
+// Launches of the attention kernels for one element type; a translation unit each (attn_f32.hip, attn_bf16.hip, attn_f16.hip)
+// instantiates attn_run.
+#pragma once
+#include "attn_kernels.h"
+
+namespace trace {
+namespace {
+
+template <typename K>
+int launch(K kernel, unsigned long long* attr, size_t lds, int threads, const AttnArgs& a, hipStream_t st, const char* what) {
+  const long grid = xcd_grid(a.items);
+  TRACE_REQUIRE(grid < 0x7fffffffL, "%s: grid of %ld workgroups", what, grid);
+  if (lds > 64 * 1024) TRACE_CHECK_HIP(ensure_dynamic_lds(attr, reinterpret_cast<const void*>(kernel), (int)lds));
+  hipLaunchKernelGGL(kernel, dim3((unsigned)grid), dim3(threads), lds, st, a);
+  return launch_status(what);
+}
+
+// Waves of a workgroup: as many as the 32-row tiles that one (batch, head) has, up to four -- a sequence of 52 steps
+// keeps two busy.
+int waves_for(int rows) { return rows <= 32 ? 1 : rows <= 64 ? 2 : 4; }
+
+template <typename T, int DP, int NW>
+int fwd(AttnArgs a, hipStream_t st) {
+  static unsigned long long attr = 0;
+  a.items = (long)((a.Lq + 32 * NW - 1) / (32 * NW)) * a.Hq * a.B;
+  const size_t lds = sizeof(T) * (64 * TileR<T, DP>::S + DP * TileX<T, 64>::S);
+  return launch(&attn_fwd_kernel<T, DP, NW>, &attr, lds, NW * 64, a, st, "attn_fwd_kernel");
+}
+
+template <typename T, int DP, int NW>
+int dq(AttnArgs a, hipStream_t st) {
+  static unsigned long long attr = 0;
+  a.items = (long)((a.Lq + 32 * NW - 1) / (32 * NW)) * a.Hq * a.B;
+  const size_t lds = sizeof(T) * (2 * 64 * TileR<T, DP>::S + DP * TileX<T, 64>::S);
+  return launch(&attn_dq_kernel<T, DP, NW>, &attr, lds, NW * 64, a, st, "attn_dq_kernel");
+}
+
+template <typename T, int DP, int NW>
+int dkv(AttnArgs a, hipStream_t st) {
+  static unsigned long long attr = 0;
+  a.items = (long)((a.Lk + 32 * NW - 1) / (32 * NW)) * a.Hk * a.B;
+  const size_t lds = sizeof(T) * 2 * (32 * TileR<T, DP>::S + DP * TileX<T, 32>::S) + 2 * 32 * sizeof(float);
+  return launch(&attn_dkv_kernel<T, DP, NW>, &attr, lds, NW * 64, a, st, "attn_dkv_kernel");
+}
+
+template <typename T, int DP>
+int few(const AttnArgs& a, hipStream_t st) {
+  int r = launch(&attn_few_kernel<T, DP>, nullptr, 0, 64, a, st, "attn_few_kernel");
+  if (r != TRACE_OK || a.splits == 1) return r;
+  const int64_t rows = (int64_t)a.B * a.Hk * a.Lq * a.G;
+  TRACE_REQUIRE(rows < 0x7fffffffL, "attn_join_kernel: grid of %lld workgroups", (long long)rows);
+  hipLaunchKernelGGL((attn_join_kernel<T, DP>), dim3((unsigned)rows), dim3(256), 0, st, a);
+  return launch_status("attn_join_kernel");
+}
+#define TRACE_ATTN_NW(FN, T, DP, W) (W == 1 ? FN<T, DP, 1>(a, st) : W == 2 ? FN<T, DP, 2>(a, st) : FN<T, DP, 4>(a, st))
+#define TRACE_ATTN_DP(FN, T, LEN)                                                      \
+  (a.D <= 32   ? TRACE_ATTN_NW(FN, T, 32, waves_for(LEN))                              \
+   : a.D <= 64 ? TRACE_ATTN_NW(FN, T, 64, waves_for(LEN))                              \
+               : TRACE_ATTN_NW(FN, T, 128, waves_for(LEN)))
+
+}  // namespace
+
+template <typename T>
+int attn_run(AttnPass pass, const AttnArgs& a, hipStream_t st) {
+  switch (pass) {
+    case AttnPass::forward: return TRACE_ATTN_DP(fwd, T, a.Lq);
+    case AttnPass::few: return a.D <= 32 ? few<T, 32>(a, st) : a.D <= 64 ? few<T, 64>(a, st) : few<T, 128>(a, st);
+    case AttnPass::dq: return TRACE_ATTN_DP(dq, T, a.Lq);
+    default: return TRACE_ATTN_DP(dkv, T, a.Lk);
+  }
+}
+
+}  // namespace trace
