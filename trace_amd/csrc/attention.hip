@@ -47,6 +47,8 @@ AttnArgs common_args(const trace_attention_desc& d) {
   return a;
 }
 
+int padded_dim(int D) { return D <= 32 ? 32 : D <= 64 ? 64 : 128; }
+
 // The form for few queries.  waves: enough to keep every CU's memory queue full (8 a CU measured best); a range has at
 // least 64 keys.
 struct FewPlan {
@@ -66,8 +68,25 @@ FewPlan few_plan(const trace_attention_desc& d) {
   p.rows = pairs * N;
   if (p.use && p.splits > 1) {
     p.ml_bytes = (p.rows * p.splits * 2 * (int64_t)sizeof(float) + 15) / 16 * 16;
-    p.bytes = p.ml_bytes + p.rows * p.splits * (d.D <= 32 ? 32 : d.D <= 64 ? 64 : 128) * (int64_t)sizeof(float);
+    p.bytes = p.ml_bytes + p.rows * p.splits * padded_dim(d.D) * (int64_t)sizeof(float);
   }
+  return p;
+}
+
+// Shares of the dk / dv kernel's queries: enough for four workgroups a CU, each with at least 16 query tiles.
+struct BackPlan {
+  int splits;
+  int64_t delta_bytes, bytes;
+};
+BackPlan back_plan(const trace_attention_desc& d) {
+  const int64_t items = (int64_t)((d.Lk + 127) / 128) * d.Hk * d.B;
+  const int64_t list = (int64_t)((d.Lq + 31) / 32) * (d.Hq / d.Hk);
+  int64_t n = items > 0 ? (1024 + items - 1) / items : 1;
+  n = n < list / 16 ? n : list / 16;
+  BackPlan p{};
+  p.splits = (int)(n < 1 ? 1 : n < 16 ? n : 16);
+  p.delta_bytes = ((int64_t)d.B * d.Hq * d.Lq * (int64_t)sizeof(float) + 15) / 16 * 16;
+  p.bytes = p.delta_bytes + (p.splits > 1 ? (int64_t)p.splits * 2 * d.B * d.Hk * d.Lk * padded_dim(d.D) * (int64_t)sizeof(float) : 0);
   return p;
 }
 
@@ -86,7 +105,7 @@ extern "C" int64_t trace_attention_workspace_bytes(const trace_attention_desc* d
   const int rc = check_desc(d, "trace_attention_workspace_bytes");
   if (rc != TRACE_OK) return rc;
   if (d->B == 0 || d->Lq == 0) return 0;
-  return backward ? (int64_t)d->B * d->Hq * d->Lq * (int64_t)sizeof(float) : few_plan(*d).bytes;
+  return backward ? back_plan(*d).bytes : few_plan(*d).bytes;
 }
 
 extern "C" int trace_attention(const trace_attention_desc* d, const void* q, const void* k, const void* v, void* out,
@@ -134,6 +153,7 @@ extern "C" int trace_attention_backward(const trace_attention_desc* d, const voi
               (long long)need);
     return TRACE_ENOMEM;
   }
+  TRACE_REQUIRE(need == 0 || aligned16(workspace), "trace_attention_backward: workspace must be 16-byte aligned");
   AttnArgs a = common_args(*d);
   Check c{*d, d->dtype == TRACE_F32 ? 4 : 2, d->D % 8 == 0};
   a.q = q; a.vq = c.view(d->q, q);
@@ -145,7 +165,10 @@ extern "C" int trace_attention_backward(const trace_attention_desc* d, const voi
   a.dk = dk; a.vdk = c.view(d->dk, dk);
   a.dv = dv; a.vdv = c.view(d->dv, dv);
   a.lse_in = lse;
+  const BackPlan plan = back_plan(*d);
   a.delta = static_cast<float*>(workspace);
+  a.splits = plan.splits;
+  a.part_o = reinterpret_cast<float*>(static_cast<char*>(workspace) + plan.delta_bytes);
   a.vec = c.vec;
   if (d->Lq > 0) {
     const int r = by_type(d->dtype, AttnPass::dq, a, (hipStream_t)stream);

@@ -34,8 +34,9 @@ struct AttnArgs {
   const unsigned char* key_mask;     // (B, Lk) or null
   long mask_stride;
   int vec;                           // every pointer and stride 16-byte aligned, D % 8 == 0
-  int splits;                        // ranges of keys (attn_few_kernel)
-  float *part_ml, *part_o;           // their partial results: (rows, splits, 2), (rows, splits, padded D)
+  int splits;                        // ranges of keys (attn_few_kernel), shares of the queries (attn_dkv_kernel)
+  float *part_ml, *part_o;           // their partial results: (rows, splits, 2), (rows, splits, padded D) or
+                                     // (splits, {dk, dv}, rows, padded D)
   long items;                        // work items of the launch
 };
 constexpr int ATTN_MAX_SPLITS = 256;
@@ -135,7 +136,7 @@ __device__ __forceinline__ long causal_start(const AttnArgs& a, int b) {
 // ---- forward ------------------------------------------------------------------------------------------------------
 // One workgroup = 32 NW queries of one head, one wave = 32 of them; the keys pass in tiles of 64.
 template <typename T, int DP, int NW>
-__global__ __launch_bounds__(NW * 64) void attn_fwd_kernel(AttnArgs a) {
+__global__ __launch_bounds__(NW * 64, sizeof(T) == 2 || DP <= 64 ? 2 : 1) void attn_fwd_kernel(AttnArgs a) {
   typedef typename Elem<T>::V8 V8;
   constexpr int KT = 64, NT = NW * 64, NC = DP / 16, ND = DP / 32;
   constexpr int UN = KT / 4 * (DP / 8), UPT = (2 * UN + NT - 1) / NT;
@@ -171,25 +172,41 @@ __global__ __launch_bounds__(NW * 64) void attn_fwd_kernel(AttnArgs a) {
 
   const T* kb = (const T*)a.k + b * a.vk.sb + hk * a.vk.sh;
   const T* vb = (const T*)a.v + b * a.vv.sb + hk * a.vv.sh;
-  Unit<T> un[UPT];
+  // The next tile is on its way in registers while this one is worked on, where that takes at most two units a thread;
+  // workgroups of fewer waves load between the barriers, and several of them share a CU.
+  constexpr bool AHEAD = UPT <= 2;
+  Unit<T> un[AHEAD ? UPT : 1];
+  auto load_unit = [&](Unit<T>& to, int n, int key0, unsigned long long bits) {
+    const int u = tid + n * NT;
+    const bool is_v = u >= UN;
+    const int w = is_v ? u - UN : u;
+    const int quad = w / (DP / 8), d = w % (DP / 8) * 8;
+    const unsigned ok = u < 2 * UN ? (unsigned)(bits >> (quad * 4)) & 15u : 0u;
+    const long sl = is_v ? a.vv.sl : a.vk.sl;
+    to.load((is_v ? vb : kb) + (long)(key0 + quad * 4) * sl + d, sl, a.D - d, ok, vec);
+  };
   auto fetch = [&](int key0, unsigned long long bits) {
+    if (AHEAD) {
 #pragma unroll
-    for (int n = 0; n < UPT; ++n) {
-      const int u = tid + n * NT;
-      const bool is_v = u >= UN;
-      const int w = is_v ? u - UN : u;
-      const int quad = w / (DP / 8), d = w % (DP / 8) * 8;
-      const unsigned ok = u < 2 * UN ? (unsigned)(bits >> (quad * 4)) & 15u : 0u;
-      const long sl = is_v ? a.vv.sl : a.vk.sl;
-      un[n].load((is_v ? vb : kb) + (long)(key0 + quad * 4) * sl + d, sl, a.D - d, ok, vec);
+      for (int n = 0; n < (AHEAD ? UPT : 1); ++n) load_unit(un[n], n, key0, bits);
     }
   };
-  auto put = [&]() {
+  auto put_unit = [&](const Unit<T>& from, int n) {
+    const int u = tid + n * NT;
+    if (u < UN) from.template put_r<DP>(kt, u);
+    else if (u < 2 * UN) from.template put_x<DP, KT>(vx, u - UN);
+  };
+  auto put = [&](int key0, unsigned long long bits) {
+    if (AHEAD) {
 #pragma unroll
-    for (int n = 0; n < UPT; ++n) {
-      const int u = tid + n * NT;
-      if (u < UN) un[n].template put_r<DP>(kt, u);
-      else if (u < 2 * UN) un[n].template put_x<DP, KT>(vx, u - UN);
+      for (int n = 0; n < (AHEAD ? UPT : 1); ++n) put_unit(un[n], n);
+    } else {
+#pragma unroll 2
+      for (int n = 0; n < UPT; ++n) {
+        Unit<T> t;
+        load_unit(t, n, key0, bits);
+        put_unit(t, n);
+      }
     }
   };
 
@@ -199,7 +216,7 @@ __global__ __launch_bounds__(NW * 64) void attn_fwd_kernel(AttnArgs a) {
   fetch(0, bits);
   for (int key0 = 0; key0 < end; key0 += KT) {
     __syncthreads();
-    put();
+    put(key0, bits);
     __syncthreads();
     const unsigned long long here = bits;
     if (key0 + KT < end) {
@@ -458,7 +475,7 @@ __global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a) {
 // One workgroup = 32 NW queries of one head, keys in tiles of KT: S^T and dP^T = V dO^T share the layout of the forward,
 // dq^T += K^T dS^T.  delta = dout . out is formed here first and left for the dk / dv kernel.
 template <typename T, int DP, int NW>
-__global__ __launch_bounds__(NW * 64) void attn_dq_kernel(AttnArgs a) {
+__global__ __launch_bounds__(NW * 64, sizeof(T) == 2 || DP <= 64 ? 2 : 1) void attn_dq_kernel(AttnArgs a) {
   typedef typename Elem<T>::V8 V8;
   constexpr int KT = 64, NT = NW * 64, NC = DP / 16, ND = DP / 32;
   constexpr int UN = KT / 4 * (DP / 8), UPT = (2 * UN + NT - 1) / NT;
@@ -502,28 +519,44 @@ __global__ __launch_bounds__(NW * 64) void attn_dq_kernel(AttnArgs a) {
   const long sees = (long)i + start;
   const T* kb = (const T*)a.k + b * a.vk.sb + hk * a.vk.sh;
   const T* vb = (const T*)a.v + b * a.vv.sb + hk * a.vv.sh;
-  Unit<T> un[UPT];
+  // The next tile is on its way in registers while this one is worked on, where that takes at most two units a thread;
+  // workgroups of fewer waves load between the barriers, and several of them share a CU.
+  constexpr bool AHEAD = UPT <= 2;
+  Unit<T> un[AHEAD ? UPT : 1];
+  auto load_unit = [&](Unit<T>& to, int n, int key0, unsigned long long bits) {
+    const int u = tid + n * NT;
+    const bool is_v = u >= UN;
+    const int w = is_v ? u - UN : u;
+    const int quad = w / (DP / 8), d = w % (DP / 8) * 8;
+    const unsigned ok = u < 2 * UN ? (unsigned)(bits >> (quad * 4)) & 15u : 0u;
+    const long sl = is_v ? a.vv.sl : a.vk.sl;
+    to.load((is_v ? vb : kb) + (long)(key0 + quad * 4) * sl + d, sl, a.D - d, ok, vec);
+  };
   auto fetch = [&](int key0, unsigned long long bits) {
+    if (AHEAD) {
 #pragma unroll
-    for (int n = 0; n < UPT; ++n) {
-      const int u = tid + n * NT;
-      const bool is_v = u >= UN;
-      const int w = is_v ? u - UN : u;
-      const int quad = w / (DP / 8), d = w % (DP / 8) * 8;
-      const unsigned ok = u < 2 * UN ? (unsigned)(bits >> (quad * 4)) & 15u : 0u;
-      const long sl = is_v ? a.vv.sl : a.vk.sl;
-      un[n].load((is_v ? vb : kb) + (long)(key0 + quad * 4) * sl + d, sl, a.D - d, ok, vec);
+      for (int n = 0; n < (AHEAD ? UPT : 1); ++n) load_unit(un[n], n, key0, bits);
     }
   };
-  auto put = [&]() {
+  auto put_unit = [&](const Unit<T>& from, int n) {
+    const int u = tid + n * NT;
+    if (u < UN) {
+      from.template put_r<DP>(kt, u);
+      from.template put_x<DP, KT>(kx, u);
+    } else if (u < 2 * UN) {
+      from.template put_r<DP>(vt, u - UN);
+    }
+  };
+  auto put = [&](int key0, unsigned long long bits) {
+    if (AHEAD) {
 #pragma unroll
-    for (int n = 0; n < UPT; ++n) {
-      const int u = tid + n * NT;
-      if (u < UN) {
-        un[n].template put_r<DP>(kt, u);
-        un[n].template put_x<DP, KT>(kx, u);
-      } else if (u < 2 * UN) {
-        un[n].template put_r<DP>(vt, u - UN);
+      for (int n = 0; n < (AHEAD ? UPT : 1); ++n) put_unit(un[n], n);
+    } else {
+#pragma unroll 2
+      for (int n = 0; n < UPT; ++n) {
+        Unit<T> t;
+        load_unit(t, n, key0, bits);
+        put_unit(t, n);
       }
     }
   };
@@ -532,7 +565,7 @@ __global__ __launch_bounds__(NW * 64) void attn_dq_kernel(AttnArgs a) {
   fetch(0, bits);
   for (int key0 = 0; key0 < end; key0 += KT) {
     __syncthreads();
-    put();
+    put(key0, bits);
     __syncthreads();
     const unsigned long long here = bits;
     if (key0 + KT < end) {
@@ -582,12 +615,18 @@ __global__ __launch_bounds__(NW * 64) void attn_dq_kernel(AttnArgs a) {
 }
 
 // ---- backward: dk, dv ------------------------------------------------------------------------------------------------
+// With few workgroups the list of (head, query tile) is cut into `splits` shares, whose fp32 results attn_sum_kernel adds in order.
+// V_LDS: 16-bit heads of 128 leave no room for the values beside both accumulators at two waves a SIMD.
+template <typename T, int DP>
+constexpr bool DKV_V_LDS = sizeof(T) == 2 && DP == 128;
+
 // One workgroup = 32 NW keys of one key head, one wave = 32 of them; the queries of every head that shares it pass in
 // tiles of 32.  S and dP = dO V^T here have queries as rows: dv^T += dO^T P, dk^T += Q^T dS.  The sums over heads
 // and queries stay in one accumulator in a fixed order: no atomics, the same bits every time.
 template <typename T, int DP, int NW>
-__global__ __launch_bounds__(NW * 64) void attn_dkv_kernel(AttnArgs a) {
+__global__ __launch_bounds__(NW * 64, sizeof(T) == 2 || DP <= 32 ? 2 : 1) void attn_dkv_kernel(AttnArgs a) {
   typedef typename Elem<T>::V8 V8;
+  constexpr bool V_LDS = DKV_V_LDS<T, DP>;
   constexpr int QT = 32, NT = NW * 64, NC = DP / 16, ND = DP / 32;
   constexpr int UN = QT / 4 * (DP / 8), UPT = (2 * UN + NT - 1) / NT;
   extern __shared__ __attribute__((aligned(16))) char lds[];
@@ -597,71 +636,91 @@ __global__ __launch_bounds__(NW * 64) void attn_dkv_kernel(AttnArgs a) {
   T* const gx = qx + DP * TileX<T, QT>::S;
   float* const lse2s = reinterpret_cast<float*>(gx + DP * TileX<T, QT>::S);
   float* const deltas = lse2s + QT;
+  T* const vt = reinterpret_cast<T*>(deltas + QT);        // V_LDS: the workgroup's values
   const long item = xcd_item(a.items);
   if (item >= a.items) return;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, col = lane & 31, half = lane >> 5;
   const int tiles = (a.Lk + 32 * NW - 1) / (32 * NW);
-  const int tile = (int)(item % tiles);                   // causal: the first keys are seen by the most queries
-  const int hk = (int)((item / tiles) % a.Hk);
-  const int b = (int)(item / tiles / a.Hk);
+  const int split = (int)(item % a.splits);
+  const int tile = (int)(item / a.splits % tiles);        // causal: the first keys are seen by the most queries
+  const int hk = (int)((item / a.splits / tiles) % a.Hk);
+  const int b = (int)(item / a.splits / tiles / a.Hk);
   const int key0 = tile * 32 * NW;
   const int j = key0 + wave * 32 + col;                   // this lane's key
   const bool vec = a.vec != 0;
   const int len = key_limit(a, b);
   const long start = causal_start(a, b);
   const bool on = j < len && (!a.key_mask || a.key_mask[(long)b * a.mask_stride + j] != 0);
-  V8 kf[NC], vf[NC];
+  V8 kf[NC], vf[V_LDS ? 1 : NC];
 #pragma unroll
   for (int c = 0; c < NC; ++c) {
     const int d = c * 16 + half * 8, n = on ? a.D - d : 0;
     kf[c] = load8<T>((const T*)a.k + b * a.vk.sb + hk * a.vk.sh + (long)j * a.vk.sl + d, n, vec);
-    vf[c] = load8<T>((const T*)a.v + b * a.vv.sb + hk * a.vv.sh + (long)j * a.vv.sl + d, n, vec);
+    const V8 t = load8<T>((const T*)a.v + b * a.vv.sb + hk * a.vv.sh + (long)j * a.vv.sl + d, n, vec);
+    // a lane reads back only what it writes here: no barrier
+    if (V_LDS) *reinterpret_cast<V8*>(vt + TileR<T, DP>::frag(wave * 32 + col, c, half)) = t;
+    else vf[V_LDS ? 0 : c] = t;
   }
   const int first = (int)max(0L, min((long)a.Lq, (long)key0 - start)) / QT * QT;      // queries before see none of these keys
   const int per_head = first < a.Lq && key0 < len ? (a.Lq - first + QT - 1) / QT : 0;
-  const int total = per_head * a.G;
+  // this workgroup's share of the (head, query tile) list
+  const long list = (long)per_head * a.G;
+  const int begin = (int)(list * split / a.splits), total = (int)(list * (split + 1) / a.splits) - begin;
   f32x16 dk[ND] = {}, dv[ND] = {};
-  Unit<T> un[UPT];
+  constexpr bool AHEAD = UPT <= 2;
+  Unit<T> un[AHEAD ? UPT : 1];
+  float sn[AHEAD ? UPT : 1][4];
   float row_lse = 0.f, row_delta = 0.f;
-  auto fetch = [&](int n_tile) {
-    const int hq = hk * a.G + n_tile / per_head;
-    const int q0 = first + n_tile % per_head * QT;
-    const float* lse = a.lse_in + ((long)b * a.Hq + hq) * a.Lq;
+  auto load_unit = [&](Unit<T>& to, float (&seen)[4], int n, int hq, int q0) {
+    const int u = tid + n * NT;
+    const bool is_g = u >= UN;
+    const int w = is_g ? u - UN : u;
+    const int quad = w / (DP / 8), d = w % (DP / 8) * 8;
+    const int left = u < 2 * UN ? a.Lq - q0 - quad * 4 : 0;
+    const unsigned ok = left >= 4 ? 15u : left > 0 ? (1u << left) - 1 : 0u;
+    const float* lse = a.lse_in + ((long)b * a.Hq + hq) * a.Lq + q0 + quad * 4;
 #pragma unroll
-    for (int n = 0; n < UPT; ++n) {
-      const int u = tid + n * NT;
-      const bool is_g = u >= UN;
-      const int w = is_g ? u - UN : u;
-      const int quad = w / (DP / 8), d = w % (DP / 8) * 8;
-      unsigned ok = 0;                                    // rows that see nothing count as absent, whatever they hold
-      if (u < 2 * UN) {
+    for (int e = 0; e < 4; ++e) seen[e] = e < left ? lse[e] : -INFINITY;
+    const long sb = is_g ? a.vdo.sb : a.vq.sb, sh = is_g ? a.vdo.sh : a.vq.sh, sl = is_g ? a.vdo.sl : a.vq.sl;
+    to.load((const T*)(is_g ? a.dout : a.q) + b * sb + hq * sh + (long)(q0 + quad * 4) * sl + d, sl, a.D - d, ok, vec);
+  };
+  auto put_unit = [&](Unit<T>& from, const float (&seen)[4], int n) {
+    const int u = tid + n * NT;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int r = q0 + quad * 4 + e;
-          if (r < a.Lq && lse[r] != -INFINITY) ok |= 1u << e;
-        }
-      }
-      const AttnView& v = is_g ? a.vdo : a.vq;
-      un[n].load((const T*)(is_g ? a.dout : a.q) + b * v.sb + hq * v.sh + (long)(q0 + quad * 4) * v.sl + d, v.sl,
-                 a.D - d, ok, vec);
-    }
-    if (tid < QT) {
-      const int r = q0 + tid;
-      const float x = r < a.Lq ? lse[r] : -INFINITY;
-      row_lse = x == -INFINITY ? INFINITY : x * LOG2E;
-      row_delta = x == -INFINITY ? 0.f : a.delta[((long)b * a.Hq + hq) * a.Lq + r];
+    for (int e = 0; e < 4; ++e)                           // rows that see nothing count as absent, whatever they hold
+      if (seen[e] == -INFINITY) from.r[e] = V8{};
+    if (u < UN) {
+      from.template put_r<DP>(qt, u);
+      from.template put_x<DP, QT>(qx, u);
+    } else if (u < 2 * UN) {
+      from.template put_r<DP>(gt, u - UN);
+      from.template put_x<DP, QT>(gx, u - UN);
     }
   };
-  auto put = [&]() {
+  auto fetch = [&](int hq, int q0) {
+    if (AHEAD) {
 #pragma unroll
-    for (int n = 0; n < UPT; ++n) {
-      const int u = tid + n * NT;
-      if (u < UN) {
-        un[n].template put_r<DP>(qt, u);
-        un[n].template put_x<DP, QT>(qx, u);
-      } else if (u < 2 * UN) {
-        un[n].template put_r<DP>(gt, u - UN);
-        un[n].template put_x<DP, QT>(gx, u - UN);
+      for (int n = 0; n < (AHEAD ? UPT : 1); ++n) load_unit(un[n], sn[n], n, hq, q0);
+    }
+    if (tid < QT) {
+      const long at = ((long)b * a.Hq + hq) * a.Lq + q0 + tid;
+      const float x = q0 + tid < a.Lq ? a.lse_in[at] : -INFINITY;
+      const float y = q0 + tid < a.Lq ? a.delta[at] : 0.f;
+      row_lse = x == -INFINITY ? INFINITY : x * LOG2E;
+      row_delta = x == -INFINITY ? 0.f : y;
+    }
+  };
+  auto put = [&](int hq, int q0) {
+    if (AHEAD) {
+#pragma unroll
+      for (int n = 0; n < (AHEAD ? UPT : 1); ++n) put_unit(un[n], sn[n], n);
+    } else {
+#pragma unroll 2
+      for (int n = 0; n < UPT; ++n) {
+        Unit<T> t;
+        float s[4];
+        load_unit(t, s, n, hq, q0);
+        put_unit(t, s, n);
       }
     }
     if (tid < QT) {
@@ -669,20 +728,33 @@ __global__ __launch_bounds__(NW * 64) void attn_dkv_kernel(AttnArgs a) {
       deltas[tid] = row_delta;
     }
   };
-  if (total > 0) fetch(0);
+  int hq_next = hk * a.G, q_next = first;                  // the tile that is fetched next
+  if (total > 0) {
+    hq_next += begin / per_head;
+    q_next += begin % per_head * QT;
+  }
+  if (total > 0) fetch(hq_next, q_next);
   for (int n_tile = 0; n_tile < total; ++n_tile) {
+    const int q0 = q_next;
     __syncthreads();
-    put();
+    put(hq_next, q0);
     __syncthreads();
-    const int q0 = first + n_tile % per_head * QT;
-    if (n_tile + 1 < total) fetch(n_tile + 1);
+    q_next += QT;
+    if (q_next >= a.Lq) {
+      q_next = first;
+      ++hq_next;
+    }
+    if (n_tile + 1 < total) fetch(hq_next, q_next);
     if ((long)key0 + wave * 32 > q0 + QT - 1 + start) continue;       // none of the wave's keys is seen
     const bool partial = (long)key0 + wave * 32 + 31 > q0 + start || !__all(on);
     f32x16 s = {}, dp = {};
 #pragma unroll
     for (int c = 0; c < NC; ++c) s = Elem<T>::mma32(frag_at<T>(qt, TileR<T, DP>::frag(col, c, half)), kf[c], s);
 #pragma unroll
-    for (int c = 0; c < NC; ++c) dp = Elem<T>::mma32(frag_at<T>(gt, TileR<T, DP>::frag(col, c, half)), vf[c], dp);
+    for (int c = 0; c < NC; ++c) {
+      const V8 v = V_LDS ? frag_at<T>(vt, TileR<T, DP>::frag(wave * 32 + col, c, half)) : vf[V_LDS ? 0 : c];
+      dp = Elem<T>::mma32(frag_at<T>(gt, TileR<T, DP>::frag(col, c, half)), v, dp);
+    }
 #pragma unroll
     for (int g = 0; g < 4; ++g) {
       const f32v4 ls = *reinterpret_cast<const f32v4*>(lse2s + 8 * g + 4 * half);
@@ -713,6 +785,20 @@ __global__ __launch_bounds__(NW * 64) void attn_dkv_kernel(AttnArgs a) {
     }
   }
   if (j >= a.Lk) return;
+  if (a.splits > 1) {
+    const long rows = (long)a.B * a.Hk * a.Lk, row = ((long)b * a.Hk + hk) * a.Lk + j;
+    float* pk = a.part_o + (2 * split * rows + row) * DP;
+    float* pv = pk + rows * DP;
+#pragma unroll
+    for (int dt = 0; dt < ND; ++dt)
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        const int d = dt * 32 + g * 8 + half * 4;
+        *reinterpret_cast<f32v4*>(pk + d) = f32v4{dk[dt][4 * g], dk[dt][4 * g + 1], dk[dt][4 * g + 2], dk[dt][4 * g + 3]};
+        *reinterpret_cast<f32v4*>(pv + d) = f32v4{dv[dt][4 * g], dv[dt][4 * g + 1], dv[dt][4 * g + 2], dv[dt][4 * g + 3]};
+      }
+    return;
+  }
   T* pk = (T*)a.dk + b * a.vdk.sb + hk * a.vdk.sh + (long)j * a.vdk.sl;
   T* pv = (T*)a.dv + b * a.vdv.sb + hk * a.vdv.sh + (long)j * a.vdv.sl;
 #pragma unroll
@@ -727,6 +813,31 @@ __global__ __launch_bounds__(NW * 64) void attn_dkv_kernel(AttnArgs a) {
       store4<T>(pk + d, w, a.D - d, vec);
       store4<T>(pv + d, x, a.D - d, vec);
     }
+}
+
+// dk and dv from the fp32 shares of the dk / dv kernel; a lane has four head elements of one key.
+template <typename T, int DP>
+__global__ __launch_bounds__(256) void attn_sum_kernel(AttnArgs a) {
+  constexpr int PER = DP / 4;
+  const long rows = (long)a.B * a.Hk * a.Lk;
+  const long at = (long)blockIdx.x * 256 + threadIdx.x, row = at / PER;
+  const int d = (int)(at % PER) * 4;
+  if (row >= rows || d >= a.D) return;
+  f32v4 dk = {}, dv = {};
+  for (int s = 0; s < a.splits; ++s) {
+    const float* p = a.part_o + (2 * s * rows + row) * DP + d;
+    const f32v4 x = *reinterpret_cast<const f32v4*>(p), y = *reinterpret_cast<const f32v4*>(p + rows * DP);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      dk[e] += x[e];
+      dv[e] += y[e];
+    }
+  }
+#pragma unroll
+  for (int e = 0; e < 4; ++e) dk[e] *= a.scale;
+  const int j = (int)(row % a.Lk), hk = (int)(row / a.Lk % a.Hk), b = (int)(row / a.Lk / a.Hk);
+  store4<T>((T*)a.dk + b * a.vdk.sb + hk * a.vdk.sh + (long)j * a.vdk.sl + d, dk, a.D - d, a.vec);
+  store4<T>((T*)a.dv + b * a.vdv.sb + hk * a.vdv.sh + (long)j * a.vdv.sl + d, dv, a.D - d, a.vec);
 }
 
 }  // namespace trace

@@ -38,9 +38,15 @@ int dq(AttnArgs a, hipStream_t st) {
 template <typename T, int DP, int NW>
 int dkv(AttnArgs a, hipStream_t st) {
   static unsigned long long attr = 0;
-  a.items = (long)((a.Lk + 32 * NW - 1) / (32 * NW)) * a.Hk * a.B;
-  const size_t lds = sizeof(T) * 2 * (32 * TileR<T, DP>::S + DP * TileX<T, 32>::S) + 2 * 32 * sizeof(float);
-  return launch(&attn_dkv_kernel<T, DP, NW>, &attr, lds, NW * 64, a, st, "attn_dkv_kernel");
+  a.items = (long)((a.Lk + 32 * NW - 1) / (32 * NW)) * a.Hk * a.B * a.splits;
+  const size_t lds = sizeof(T) * 2 * (32 * TileR<T, DP>::S + DP * TileX<T, 32>::S) + 2 * 32 * sizeof(float) +
+                     (DKV_V_LDS<T, DP> ? sizeof(T) * 32 * NW * TileR<T, DP>::S : 0);
+  const int r = launch(&attn_dkv_kernel<T, DP, NW>, &attr, lds, NW * 64, a, st, "attn_dkv_kernel");
+  if (r != TRACE_OK || a.splits == 1) return r;
+  const long grid = ((long)a.B * a.Hk * a.Lk * (DP / 4) + 255) / 256;
+  TRACE_REQUIRE(grid < 0x7fffffffL, "attn_sum_kernel: grid of %ld workgroups", grid);
+  hipLaunchKernelGGL((attn_sum_kernel<T, DP>), dim3((unsigned)grid), dim3(256), 0, st, a);
+  return launch_status("attn_sum_kernel");
 }
 
 template <typename T, int DP>
