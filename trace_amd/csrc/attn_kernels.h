@@ -73,10 +73,27 @@ struct TileX {
 template <typename T>
 struct Unit {
   typename Elem<T>::V8 r[4];
-  // p: element (token 0 of the unit, first head element); n: head elements left of D; valid: bit i = token i exists
-  __device__ __forceinline__ void load(const T* p, long sl, int n, unsigned valid, bool vec) {
+  // Tokens row .. row + 3 of a head at base, head elements d .. d + 7.  valid: bit i = token row + i counts (others become
+  // zero); rows: tokens that exist (>= 1); whole: uniform, all of the tile counts and vec holds.  With 16-byte loads every lane
+  // loads, absent tokens from the last one there is: no branches around loads.
+  __device__ __forceinline__ void load(const T* base, long sl, int row, int rows, int d, int D, unsigned valid, bool vec,
+                                       bool whole) {
+    typedef typename Elem<T>::V8 V8;
+    if (whole) {
+      const T* p = base + (long)row * sl + d;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) r[i] = load8<T>(p + i * sl, (valid >> i) & 1 ? n : 0, vec);
+      for (int i = 0; i < 4; ++i) r[i] = *reinterpret_cast<const V8*>(p + i * sl);
+    } else if (vec) {
+      const T* p = base + (d < D ? d : 0);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) r[i] = *reinterpret_cast<const V8*>(p + (long)min(row + i, rows - 1) * sl);
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (d >= D || !((valid >> i) & 1)) r[i] = V8{};
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) r[i] = load8<T>(base + (long)(row + i) * sl + d, (valid >> i) & 1 ? D - d : 0, false);
+    }
   }
   template <int DP>
   __device__ __forceinline__ void put_r(T* tile, int u) const {
@@ -172,10 +189,7 @@ __global__ __launch_bounds__(NW * 64, sizeof(T) == 2 || DP <= 64 ? 2 : 1) void a
 
   const T* kb = (const T*)a.k + b * a.vk.sb + hk * a.vk.sh;
   const T* vb = (const T*)a.v + b * a.vv.sb + hk * a.vv.sh;
-  // The next tile is on its way in registers while this one is worked on, where that takes at most two units a thread;
-  // workgroups of fewer waves load between the barriers, and several of them share a CU.
-  constexpr bool AHEAD = UPT <= 2;
-  Unit<T> un[AHEAD ? UPT : 1];
+  const bool whole = vec && a.D == DP && 2 * UN % NT == 0;
   auto load_unit = [&](Unit<T>& to, int n, int key0, unsigned long long bits) {
     const int u = tid + n * NT;
     const bool is_v = u >= UN;
@@ -183,47 +197,32 @@ __global__ __launch_bounds__(NW * 64, sizeof(T) == 2 || DP <= 64 ? 2 : 1) void a
     const int quad = w / (DP / 8), d = w % (DP / 8) * 8;
     const unsigned ok = u < 2 * UN ? (unsigned)(bits >> (quad * 4)) & 15u : 0u;
     const long sl = is_v ? a.vv.sl : a.vk.sl;
-    to.load((is_v ? vb : kb) + (long)(key0 + quad * 4) * sl + d, sl, a.D - d, ok, vec);
-  };
-  auto fetch = [&](int key0, unsigned long long bits) {
-    if (AHEAD) {
-#pragma unroll
-      for (int n = 0; n < (AHEAD ? UPT : 1); ++n) load_unit(un[n], n, key0, bits);
-    }
+    to.load(is_v ? vb : kb, sl, key0 + quad * 4, a.Lk, d, a.D, ok, vec, whole && bits == ~0ull);
   };
   auto put_unit = [&](const Unit<T>& from, int n) {
     const int u = tid + n * NT;
     if (u < UN) from.template put_r<DP>(kt, u);
     else if (u < 2 * UN) from.template put_x<DP, KT>(vx, u - UN);
   };
-  auto put = [&](int key0, unsigned long long bits) {
-    if (AHEAD) {
-#pragma unroll
-      for (int n = 0; n < (AHEAD ? UPT : 1); ++n) put_unit(un[n], n);
-    } else {
+  auto stage = [&](int key0, unsigned long long bits) {
 #pragma unroll 2
-      for (int n = 0; n < UPT; ++n) {
-        Unit<T> t;
-        load_unit(t, n, key0, bits);
-        put_unit(t, n);
-      }
+    for (int n = 0; n < UPT; ++n) {
+      Unit<T> t;
+      load_unit(t, n, key0, bits);
+      put_unit(t, n);
     }
   };
 
   f32x16 o[ND] = {};
   float m = -INFINITY, l = 0.f;                            // l: the sum over this lane half's keys
   unsigned long long bits = key_bits(a, b, 0, end);
-  fetch(0, bits);
   for (int key0 = 0; key0 < end; key0 += KT) {
-    __syncthreads();
-    put(key0, bits);
-    __syncthreads();
     const unsigned long long here = bits;
-    if (key0 + KT < end) {
-      bits = key_bits(a, b, key0 + KT, end);
-      fetch(key0 + KT, bits);
-    }
-    if (here == 0ull) continue;
+    if (key0 + KT < end) bits = key_bits(a, b, key0 + KT, end);
+    if (here == 0ull) continue;                            // the same in every wave
+    __syncthreads();
+    stage(key0, here);
+    __syncthreads();
     f32x16 s[2] = {};
 #pragma unroll
     for (int t = 0; t < 2; ++t)
@@ -231,7 +230,7 @@ __global__ __launch_bounds__(NW * 64, sizeof(T) == 2 || DP <= 64 ? 2 : 1) void a
       for (int c = 0; c < NC; ++c) s[t] = Elem<T>::mma32(frag_at<T>(kt, TileR<T, DP>::frag(t * 32 + col, c, half)), qf[c], s[t]);
     if (here != ~0ull || key0 + KT - 1 > sees - col) {     // sees - col: what the wave's first query sees
       const unsigned long long mine = here >> (4 * half);
-      const long room = sees - key0 - 4 * half;
+      const int room = (int)max(-64L, min(64L, sees - key0)) - 4 * half;
 #pragma unroll
       for (int t = 0; t < 2; ++t)
 #pragma unroll
@@ -327,6 +326,7 @@ __global__ __launch_bounds__(64) void attn_few_kernel(AttnArgs a) {
   const T* vb = (const T*)a.v + b * a.vv.sb + hk * a.vv.sh;
   V8 kf[NC];
   Unit<T> un[UPT];
+  const bool whole = vec && a.D == DP && KT / 4 * (DP / 8) % 64 == 0;
   auto fetch = [&](int key0, unsigned bits) {
     const int key = key0 + col;
     const T* p = kb + (long)key * a.vk.sl;
@@ -337,13 +337,13 @@ __global__ __launch_bounds__(64) void attn_few_kernel(AttnArgs a) {
     for (int m = 0; m < UPT; ++m) {
       const int u = lane + m * 64, quad = u / (DP / 8), d = u % (DP / 8) * 8;
       const unsigned ok = quad < KT / 4 ? (bits >> (quad * 4)) & 15u : 0u;
-      un[m].load(vb + (long)(key0 + quad * 4) * a.vv.sl + d, a.vv.sl, a.D - d, ok, vec);
+      un[m].load(vb, a.vv.sl, key0 + quad * 4, a.Lk, d, a.D, ok, vec, whole && bits == ~0u);
     }
   };
   f32x16 o[ND] = {};
   float m = -INFINITY, l = 0.f;
   unsigned bits = (unsigned)key_bits(a, b, from, end);
-  fetch(from, bits);
+  if (from < end) fetch(from, bits);                        // an empty range may have no memory behind it
   for (int key0 = from; key0 < end; key0 += KT) {
     const unsigned here = bits;
     f32x16 s = {};
@@ -363,7 +363,7 @@ __global__ __launch_bounds__(64) void attn_few_kernel(AttnArgs a) {
     if (here == 0u) continue;
     if (here != ~0u || key0 + KT - 1 > start) {              // start: what query 0 sees
       const unsigned mine = here >> (4 * half);
-      const long room = sees - key0 - 4 * half;
+      const int room = (int)max(-64L, min(64L, sees - key0)) - 4 * half;
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
         const int key = 8 * (r / 4) + r % 4;
@@ -519,10 +519,7 @@ __global__ __launch_bounds__(NW * 64, sizeof(T) == 2 || DP <= 64 ? 2 : 1) void a
   const long sees = (long)i + start;
   const T* kb = (const T*)a.k + b * a.vk.sb + hk * a.vk.sh;
   const T* vb = (const T*)a.v + b * a.vv.sb + hk * a.vv.sh;
-  // The next tile is on its way in registers while this one is worked on, where that takes at most two units a thread;
-  // workgroups of fewer waves load between the barriers, and several of them share a CU.
-  constexpr bool AHEAD = UPT <= 2;
-  Unit<T> un[AHEAD ? UPT : 1];
+  const bool whole = vec && a.D == DP && 2 * UN % NT == 0;
   auto load_unit = [&](Unit<T>& to, int n, int key0, unsigned long long bits) {
     const int u = tid + n * NT;
     const bool is_v = u >= UN;
@@ -530,13 +527,7 @@ __global__ __launch_bounds__(NW * 64, sizeof(T) == 2 || DP <= 64 ? 2 : 1) void a
     const int quad = w / (DP / 8), d = w % (DP / 8) * 8;
     const unsigned ok = u < 2 * UN ? (unsigned)(bits >> (quad * 4)) & 15u : 0u;
     const long sl = is_v ? a.vv.sl : a.vk.sl;
-    to.load((is_v ? vb : kb) + (long)(key0 + quad * 4) * sl + d, sl, a.D - d, ok, vec);
-  };
-  auto fetch = [&](int key0, unsigned long long bits) {
-    if (AHEAD) {
-#pragma unroll
-      for (int n = 0; n < (AHEAD ? UPT : 1); ++n) load_unit(un[n], n, key0, bits);
-    }
+    to.load(is_v ? vb : kb, sl, key0 + quad * 4, a.Lk, d, a.D, ok, vec, whole && bits == ~0ull);
   };
   auto put_unit = [&](const Unit<T>& from, int n) {
     const int u = tid + n * NT;
@@ -547,32 +538,23 @@ __global__ __launch_bounds__(NW * 64, sizeof(T) == 2 || DP <= 64 ? 2 : 1) void a
       from.template put_r<DP>(vt, u - UN);
     }
   };
-  auto put = [&](int key0, unsigned long long bits) {
-    if (AHEAD) {
-#pragma unroll
-      for (int n = 0; n < (AHEAD ? UPT : 1); ++n) put_unit(un[n], n);
-    } else {
+  auto stage = [&](int key0, unsigned long long bits) {
 #pragma unroll 2
-      for (int n = 0; n < UPT; ++n) {
-        Unit<T> t;
-        load_unit(t, n, key0, bits);
-        put_unit(t, n);
-      }
+    for (int n = 0; n < UPT; ++n) {
+      Unit<T> t;
+      load_unit(t, n, key0, bits);
+      put_unit(t, n);
     }
   };
   f32x16 acc[ND] = {};
   unsigned long long bits = key_bits(a, b, 0, end);
-  fetch(0, bits);
   for (int key0 = 0; key0 < end; key0 += KT) {
-    __syncthreads();
-    put(key0, bits);
-    __syncthreads();
     const unsigned long long here = bits;
-    if (key0 + KT < end) {
-      bits = key_bits(a, b, key0 + KT, end);
-      fetch(key0 + KT, bits);
-    }
-    if (here == 0ull) continue;
+    if (key0 + KT < end) bits = key_bits(a, b, key0 + KT, end);
+    if (here == 0ull) continue;                            // the same in every wave
+    __syncthreads();
+    stage(key0, here);
+    __syncthreads();
     const bool partial = here != ~0ull || key0 + KT - 1 > sees - col;
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
@@ -585,7 +567,7 @@ __global__ __launch_bounds__(NW * 64, sizeof(T) == 2 || DP <= 64 ? 2 : 1) void a
       for (int r = 0; r < 16; ++r) s[r] = __builtin_amdgcn_exp2f(fmaf(s[r], a.scale_log2, -lse2)) * (dp[r] - delta);
       if (partial) {
         const unsigned long long mine = here >> (4 * half);
-        const long room = sees - key0 - 4 * half;
+        const int room = (int)max(-64L, min(64L, sees - key0)) - 4 * half;
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
           const int key = t * 32 + 8 * (r / 4) + r % 4;
@@ -624,7 +606,7 @@ constexpr bool DKV_V_LDS = sizeof(T) == 2 && DP == 128;
 // tiles of 32.  S and dP = dO V^T here have queries as rows: dv^T += dO^T P, dk^T += Q^T dS.  The sums over heads
 // and queries stay in one accumulator in a fixed order: no atomics, the same bits every time.
 template <typename T, int DP, int NW>
-__global__ __launch_bounds__(NW * 64, sizeof(T) == 2 || DP <= 32 ? 2 : 1) void attn_dkv_kernel(AttnArgs a) {
+__global__ __launch_bounds__(NW * 64, sizeof(T) == 2 || DP <= 64 ? 2 : 1) void attn_dkv_kernel(AttnArgs a) {
   typedef typename Elem<T>::V8 V8;
   constexpr bool V_LDS = DKV_V_LDS<T, DP>;
   constexpr int QT = 32, NT = NW * 64, NC = DP / 16, ND = DP / 32;
@@ -661,16 +643,14 @@ __global__ __launch_bounds__(NW * 64, sizeof(T) == 2 || DP <= 32 ? 2 : 1) void a
     if (V_LDS) *reinterpret_cast<V8*>(vt + TileR<T, DP>::frag(wave * 32 + col, c, half)) = t;
     else vf[V_LDS ? 0 : c] = t;
   }
+  const bool all_on = __all(on);
   const int first = (int)max(0L, min((long)a.Lq, (long)key0 - start)) / QT * QT;      // queries before see none of these keys
   const int per_head = first < a.Lq && key0 < len ? (a.Lq - first + QT - 1) / QT : 0;
   // this workgroup's share of the (head, query tile) list
   const long list = (long)per_head * a.G;
   const int begin = (int)(list * split / a.splits), total = (int)(list * (split + 1) / a.splits) - begin;
   f32x16 dk[ND] = {}, dv[ND] = {};
-  constexpr bool AHEAD = UPT <= 2;
-  Unit<T> un[AHEAD ? UPT : 1];
-  float sn[AHEAD ? UPT : 1][4];
-  float row_lse = 0.f, row_delta = 0.f;
+  const bool whole = vec && a.D == DP && 2 * UN % NT == 0;
   auto load_unit = [&](Unit<T>& to, float (&seen)[4], int n, int hq, int q0) {
     const int u = tid + n * NT;
     const bool is_g = u >= UN;
@@ -682,7 +662,8 @@ __global__ __launch_bounds__(NW * 64, sizeof(T) == 2 || DP <= 32 ? 2 : 1) void a
 #pragma unroll
     for (int e = 0; e < 4; ++e) seen[e] = e < left ? lse[e] : -INFINITY;
     const long sb = is_g ? a.vdo.sb : a.vq.sb, sh = is_g ? a.vdo.sh : a.vq.sh, sl = is_g ? a.vdo.sl : a.vq.sl;
-    to.load((const T*)(is_g ? a.dout : a.q) + b * sb + hq * sh + (long)(q0 + quad * 4) * sl + d, sl, a.D - d, ok, vec);
+    to.load((const T*)(is_g ? a.dout : a.q) + b * sb + hq * sh, sl, q0 + quad * 4, a.Lq, d, a.D, ok, vec,
+            whole && q0 + QT <= a.Lq);
   };
   auto put_unit = [&](Unit<T>& from, const float (&seen)[4], int n) {
     const int u = tid + n * NT;
@@ -697,56 +678,39 @@ __global__ __launch_bounds__(NW * 64, sizeof(T) == 2 || DP <= 32 ? 2 : 1) void a
       from.template put_x<DP, QT>(gx, u - UN);
     }
   };
-  auto fetch = [&](int hq, int q0) {
-    if (AHEAD) {
-#pragma unroll
-      for (int n = 0; n < (AHEAD ? UPT : 1); ++n) load_unit(un[n], sn[n], n, hq, q0);
+  auto stage = [&](int hq, int q0) {
+#pragma unroll 2
+    for (int n = 0; n < UPT; ++n) {
+      Unit<T> t;
+      float s[4];
+      load_unit(t, s, n, hq, q0);
+      put_unit(t, s, n);
     }
     if (tid < QT) {
       const long at = ((long)b * a.Hq + hq) * a.Lq + q0 + tid;
       const float x = q0 + tid < a.Lq ? a.lse_in[at] : -INFINITY;
       const float y = q0 + tid < a.Lq ? a.delta[at] : 0.f;
-      row_lse = x == -INFINITY ? INFINITY : x * LOG2E;
-      row_delta = x == -INFINITY ? 0.f : y;
+      lse2s[tid] = x == -INFINITY ? INFINITY : x * LOG2E;
+      deltas[tid] = x == -INFINITY ? 0.f : y;
     }
   };
-  auto put = [&](int hq, int q0) {
-    if (AHEAD) {
-#pragma unroll
-      for (int n = 0; n < (AHEAD ? UPT : 1); ++n) put_unit(un[n], sn[n], n);
-    } else {
-#pragma unroll 2
-      for (int n = 0; n < UPT; ++n) {
-        Unit<T> t;
-        float s[4];
-        load_unit(t, s, n, hq, q0);
-        put_unit(t, s, n);
-      }
-    }
-    if (tid < QT) {
-      lse2s[tid] = row_lse;
-      deltas[tid] = row_delta;
-    }
-  };
-  int hq_next = hk * a.G, q_next = first;                  // the tile that is fetched next
+  int hq = hk * a.G, q0 = first;
   if (total > 0) {
-    hq_next += begin / per_head;
-    q_next += begin % per_head * QT;
+    hq += begin / per_head;
+    q0 += begin % per_head * QT;
   }
-  if (total > 0) fetch(hq_next, q_next);
-  for (int n_tile = 0; n_tile < total; ++n_tile) {
-    const int q0 = q_next;
-    __syncthreads();
-    put(hq_next, q0);
-    __syncthreads();
-    q_next += QT;
-    if (q_next >= a.Lq) {
-      q_next = first;
-      ++hq_next;
+  for (int n_tile = 0; n_tile < total; ++n_tile, q0 += QT) {
+    if (q0 >= a.Lq) {
+      q0 = first;
+      ++hq;
     }
-    if (n_tile + 1 < total) fetch(hq_next, q_next);
+    __syncthreads();
+    stage(hq, q0);
+    __syncthreads();
     if ((long)key0 + wave * 32 > q0 + QT - 1 + start) continue;       // none of the wave's keys is seen
-    const bool partial = (long)key0 + wave * 32 + 31 > q0 + start || !__all(on);
+    const bool partial = (long)key0 + wave * 32 + 31 > q0 + start || !all_on;
+    // rows of the tile before this one do not see the lane's key
+    const int sees_from = on ? (int)max(-64L, min(64L, j - start - q0)) - 4 * half : 64;
     f32x16 s = {}, dp = {};
 #pragma unroll
     for (int c = 0; c < NC; ++c) s = Elem<T>::mma32(frag_at<T>(qt, TileR<T, DP>::frag(col, c, half)), kf[c], s);
@@ -764,7 +728,7 @@ __global__ __launch_bounds__(NW * 64, sizeof(T) == 2 || DP <= 32 ? 2 : 1) void a
         const int r = 4 * g + e;
         float p = __builtin_amdgcn_exp2f(fmaf(s[r], a.scale_log2, -ls[e]));
         float ds = p * (dp[r] - de[e]);
-        if (partial && (!on || (long)j > (long)q0 + 8 * g + 4 * half + e + start)) p = ds = 0.f;
+        if (partial && 8 * g + e < sees_from) p = ds = 0.f;
         s[r] = p;
         dp[r] = ds;
       }

@@ -44,11 +44,14 @@ template <> struct Elem<_Float16> {
   }
 };
 
-// Eight elements at p, of which the first n (<= 8) exist; the others are zero.  vec: p is 16-byte aligned.
+// Eight elements at p, of which the first n exist; the others are zero.  vec: p is 16-byte aligned, and n a multiple of 8.
 template <typename T>
 __device__ __forceinline__ typename Elem<T>::V8 load8(const T* p, int n, bool vec) {
-  typename Elem<T>::V8 v;
-  if (vec && n >= 8) return *reinterpret_cast<const typename Elem<T>::V8*>(p);
+  typename Elem<T>::V8 v = {};
+  if (vec) {
+    if (n > 0) v = *reinterpret_cast<const typename Elem<T>::V8*>(p);
+    return v;
+  }
 #pragma unroll
   for (int i = 0; i < 8; ++i) v[i] = i < n ? p[i] : (T)0.f;
   return v;
