@@ -75,6 +75,7 @@ FewPlan few_plan(const trace_attention_desc& d) {
 
 // Shares of the dk / dv kernel's queries: enough for four workgroups a CU, each with at least 16 query tiles.
 struct BackPlan {
+  bool whole;                        // short sequences: one kernel, no workspace
   int splits;
   int64_t delta_bytes, bytes;
 };
@@ -84,6 +85,8 @@ BackPlan back_plan(const trace_attention_desc& d) {
   int64_t n = items > 0 ? (1024 + items - 1) / items : 1;
   n = n < list / 16 ? n : list / 16;
   BackPlan p{};
+  p.whole = d.Lq >= 1 && d.Lk >= 1 && d.Lq <= 64 && d.Lk <= 64;
+  if (p.whole) return p;
   p.splits = (int)(n < 1 ? 1 : n < 16 ? n : 16);
   p.delta_bytes = ((int64_t)d.B * d.Hq * d.Lq * (int64_t)sizeof(float) + 15) / 16 * 16;
   p.bytes = p.delta_bytes + (p.splits > 1 ? (int64_t)p.splits * 2 * d.B * d.Hk * d.Lk * padded_dim(d.D) * (int64_t)sizeof(float) : 0);
@@ -170,6 +173,7 @@ extern "C" int trace_attention_backward(const trace_attention_desc* d, const voi
   a.splits = plan.splits;
   a.part_o = reinterpret_cast<float*>(static_cast<char*>(workspace) + plan.delta_bytes);
   a.vec = c.vec;
+  if (plan.whole) return by_type(d->dtype, AttnPass::short_backward, a, (hipStream_t)stream);
   if (d->Lq > 0) {
     const int r = by_type(d->dtype, AttnPass::dq, a, (hipStream_t)stream);
     if (r != TRACE_OK) return r;

@@ -23,7 +23,7 @@ template <typename T, int DP, int NW>
 int fwd(AttnArgs a, hipStream_t st) {
   static unsigned long long attr = 0;
   a.items = (long)((a.Lq + 32 * NW - 1) / (32 * NW)) * a.Hq * a.B;
-  const size_t lds = sizeof(T) * (64 * TileR<T, DP>::S + DP * TileX<T, 64>::S);
+  const size_t lds = sizeof(T) * (KEY_TILE<T> * TileR<T, DP>::S + DP * TileX<T, KEY_TILE<T>>::S);
   return launch(&attn_fwd_kernel<T, DP, NW>, &attr, lds, NW * 64, a, st, "attn_fwd_kernel");
 }
 
@@ -31,7 +31,7 @@ template <typename T, int DP, int NW>
 int dq(AttnArgs a, hipStream_t st) {
   static unsigned long long attr = 0;
   a.items = (long)((a.Lq + 32 * NW - 1) / (32 * NW)) * a.Hq * a.B;
-  const size_t lds = sizeof(T) * (2 * 64 * TileR<T, DP>::S + DP * TileX<T, 64>::S);
+  const size_t lds = sizeof(T) * (2 * KEY_TILE<T> * TileR<T, DP>::S + DP * TileX<T, KEY_TILE<T>>::S);
   return launch(&attn_dq_kernel<T, DP, NW>, &attr, lds, NW * 64, a, st, "attn_dq_kernel");
 }
 
@@ -58,6 +58,19 @@ int few(const AttnArgs& a, hipStream_t st) {
   hipLaunchKernelGGL((attn_join_kernel<T, DP>), dim3((unsigned)rows), dim3(256), 0, st, a);
   return launch_status("attn_join_kernel");
 }
+template <typename T, int DP, int QB, int KB>
+int short_backward(AttnArgs a, hipStream_t st) {
+  static unsigned long long attr = 0;
+  a.items = (long)a.Hk * a.B;
+  const size_t lds = sizeof(T) * ((2 * QB + KB) * 32 * TileN<T, DP>::S + 32 * QB * TileN<T, 32 * KB>::S);
+  return launch(&attn_short_backward_kernel<T, DP, QB, KB>, &attr, lds, QB * KB * 64, a, st, "attn_short_backward_kernel");
+}
+template <typename T, int DP>
+int short_blocks(const AttnArgs& a, hipStream_t st) {
+  if (a.Lq <= 32) return a.Lk <= 32 ? short_backward<T, DP, 1, 1>(a, st) : short_backward<T, DP, 1, 2>(a, st);
+  return a.Lk <= 32 ? short_backward<T, DP, 2, 1>(a, st) : short_backward<T, DP, 2, 2>(a, st);
+}
+
 #define TRACE_ATTN_NW(FN, T, DP, W) (W == 1 ? FN<T, DP, 1>(a, st) : W == 2 ? FN<T, DP, 2>(a, st) : FN<T, DP, 4>(a, st))
 #define TRACE_ATTN_DP(FN, T, LEN)                                                      \
   (a.D <= 32   ? TRACE_ATTN_NW(FN, T, 32, waves_for(LEN))                              \
@@ -71,6 +84,8 @@ int attn_run(AttnPass pass, const AttnArgs& a, hipStream_t st) {
   switch (pass) {
     case AttnPass::forward: return TRACE_ATTN_DP(fwd, T, a.Lq);
     case AttnPass::few: return a.D <= 32 ? few<T, 32>(a, st) : a.D <= 64 ? few<T, 64>(a, st) : few<T, 128>(a, st);
+    case AttnPass::short_backward:
+      return a.D <= 32 ? short_blocks<T, 32>(a, st) : a.D <= 64 ? short_blocks<T, 64>(a, st) : short_blocks<T, 128>(a, st);
     case AttnPass::dq: return TRACE_ATTN_DP(dq, T, a.Lq);
     default: return TRACE_ATTN_DP(dkv, T, a.Lk);
   }
