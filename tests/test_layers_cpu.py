@@ -169,7 +169,9 @@ def test_c_entries_refuse_bad_descriptors():
     d = attention()
     assert L.trace_attention(None, p, p, p, p, p, None, 0, None) == EINVAL and "null" in _err(L)
     assert L.trace_attention(C.byref(d), p, None, p, p, p, None, 0, None) == EINVAL and "null" in _err(L)
-    assert L.trace_attention_backward(C.byref(d), p, p, p, p, p, p, p, p, p, None, 0, None) == ENOMEM
+    long = attention(Lq=100, Lk=100)                         # a call that needs a workspace
+    assert L.trace_attention_workspace_bytes(C.byref(long), 1) >= 400
+    assert L.trace_attention_backward(C.byref(long), p, p, p, p, p, p, p, p, p, None, 0, None) == ENOMEM
     assert "workspace" in _err(L)
     assert L.trace_attention(C.byref(attention(B=0)), None, None, None, None, None, None, 0, None) == 0
 

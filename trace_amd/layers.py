@@ -18,28 +18,33 @@ _DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 _NORMS = {"rms": 0, "layer": 1}
 
 
-def _need(ok, text, *args):
-    if not ok:
-        raise ValueError(text % args if args else text)
+def _refuse(text, *args):
+    raise ValueError(text % args if args else text)
 
 
-def _check(name, t, like=None, dtype=None, shape=None, dims=None):
-    """A tensor that a kernel can take: its type, device and shape, the innermost dimension contiguous."""
-    _need(isinstance(t, torch.Tensor), "%s must be a tensor", name)
-    _need(not (t.requires_grad and torch.is_grad_enabled()),
-          "%s requires grad: these operators record nothing for autograd; call them under torch.no_grad() and use their "
-          "backward functions", name)
+def _check(name, t, dtype=None, device=None, shape=None, dims=None):
+    """Refuses what a kernel cannot take: another type (dtype None: one of the three), device or shape, an innermost
+    dimension that is not contiguous, a tensor that autograd would have to record.  (Plain ifs: a small call is bound by its
+    time on the host.)"""
+    if not isinstance(t, torch.Tensor):
+        _refuse("%s must be a tensor", name)
+    if t.requires_grad and torch.is_grad_enabled():
+        _refuse("%s requires grad: these operators record nothing for autograd; call them under torch.no_grad() and use "
+                "their backward functions", name)
     if dtype is None:
-        _need(t.dtype in _DTYPES, "%s has type %s (float32, bfloat16 or float16)", name, t.dtype)
-    else:
-        _need(t.dtype == dtype, "%s has type %s, expected %s", name, t.dtype, dtype)
-    _need(like is None or t.device == like.device, "%s is on %s, expected %s", name, t.device,
-          like.device if like is not None else None)
-    if shape is not None:
-        _need(tuple(t.shape) == tuple(shape), "%s has shape %s, expected %s", name, tuple(t.shape), tuple(shape))
-    if dims is not None:
-        _need(t.dim() == dims, "%s has %d dimensions, expected %d", name, t.dim(), dims)
-    _need(t.dim() == 0 or t.shape[-1] <= 1 or t.stride(-1) == 1, "the last dimension of %s must be contiguous", name)
+        if t.dtype not in _DTYPES:
+            _refuse("%s has type %s (float32, bfloat16 or float16)", name, t.dtype)
+    elif t.dtype is not dtype:
+        _refuse("%s has type %s, expected %s", name, t.dtype, dtype)
+    if device is not None and t.device != device:
+        _refuse("%s is on %s, expected %s", name, t.device, device)
+    s = t.shape
+    if shape is not None and s != shape:
+        _refuse("%s has shape %s, expected %s", name, tuple(s), tuple(shape))
+    if dims is not None and len(s) != dims:
+        _refuse("%s has %d dimensions, expected %d", name, len(s), dims)
+    if s and s[-1] > 1 and t.stride(-1) != 1:
+        _refuse("the last dimension of %s must be contiguous", name)
 
 
 def _gpu(t):
@@ -56,7 +61,8 @@ def _enqueue(what, device, *args):
     else:
         with torch.cuda.device(device):
             rc = fn(*args, torch.cuda.current_stream(device).cuda_stream)
-    _cabi.check(rc, what)
+    if rc:
+        _cabi.check(rc, what)
 
 
 def _at(t):
@@ -67,27 +73,39 @@ def _at(t):
 
 def _attention_desc(q, k, v, causal, query_start, key_lengths, key_mask, scale, rest):
     _check("q", q, dims=4)
-    _check("k", k, like=q, dtype=q.dtype, dims=4)
+    dtype, device = q.dtype, q.device
+    _check("k", k, dtype, device, dims=4)
     B, Lq, Hq, D = q.shape
-    Lk, Hk = k.shape[1], k.shape[2]
-    _need(1 <= D <= 128, "head dimension %d unsupported (1..128)", D)
-    _need(tuple(k.shape) == (B, Lk, Hk, D), "k has shape %s, q %s", tuple(k.shape), tuple(q.shape))
-    _check("v", v, like=q, dtype=q.dtype, shape=k.shape)
-    _need(Hk >= 1 and Hq >= 1 and Hq % Hk == 0, "%d query heads cannot share %d key heads", Hq, Hk)
-    _need(max(Lq, Lk) <= 1 << 30, "more than 2^30 tokens")
+    _, Lk, Hk, _ = k.shape
+    if not 1 <= D <= 128:
+        _refuse("head dimension %d unsupported (1..128)", D)
+    if k.shape != (B, Lk, Hk, D):
+        _refuse("k has shape %s, q %s", tuple(k.shape), tuple(q.shape))
+    _check("v", v, dtype, device, k.shape)
+    if Hk < 1 or Hq < 1 or Hq % Hk:
+        _refuse("%d query heads cannot share %d key heads", Hq, Hk)
+    if Lq > 1 << 30 or Lk > 1 << 30:
+        _refuse("more than 2^30 tokens")
     scale = D ** -0.5 if scale is None else float(scale)
-    _need(math.isfinite(scale) and scale > 0, "scale %g must be positive and finite", scale)
-    _need(query_start is None or causal, "query_start has a meaning for causal attention only")
-    for name, t in (("query_start", query_start), ("key_lengths", key_lengths)):
-        if t is not None:
-            _check(name, t, like=q, dtype=torch.int32, shape=(B,))
+    if not (math.isfinite(scale) and scale > 0):
+        _refuse("scale %g must be positive and finite", scale)
+    start = lengths = mask = None
+    if query_start is not None:
+        if not causal:
+            _refuse("query_start has a meaning for causal attention only")
+        _check("query_start", query_start, torch.int32, device, (B,))
+        start = query_start.data_ptr()
+    if key_lengths is not None:
+        _check("key_lengths", key_lengths, torch.int32, device, (B,))
+        lengths = key_lengths.data_ptr()
     if key_mask is not None:
-        _check("key_mask", key_mask, like=q, dtype=torch.bool, shape=(B, Lk))
-    strides = []
-    for t in (q, k, v) + rest:
+        _check("key_mask", key_mask, torch.bool, device, (B, Lk))
+        mask = key_mask.data_ptr()
+    strides = q.stride()[:3] + k.stride()[:3] + v.stride()[:3]
+    for t in rest:
         strides += t.stride()[:3]
-    return _cabi.AttentionDesc(_DTYPES[q.dtype], B, Lq, Lk, Hq, Hk, D, scale, 1 if causal else 0, _at(query_start),
-                               _at(key_lengths), _at(key_mask), 0 if key_mask is None else key_mask.stride(0), *strides)
+    return _cabi.AttentionDesc(_DTYPES[dtype], B, Lq, Lk, Hq, Hk, D, scale, 1 if causal else 0, start, lengths, mask,
+                               0 if mask is None else key_mask.stride(0), *strides)
 
 
 def _workspace(desc, backward, device):
@@ -111,12 +129,13 @@ def attention(q, k, v, causal=False, query_start=None, key_lengths=None, key_mas
     needs.  A query that sees no key gets 0 and -inf."""
     desc = _attention_desc(q, k, v, causal, query_start, key_lengths, key_mask, scale, ())
     _gpu(q)
+    device = q.device
     B, Lq, Hq, D = q.shape
-    out = torch.empty(B, Lq, Hq, D, dtype=q.dtype, device=q.device)
-    lse = torch.empty(B, Hq, Lq, dtype=torch.float32, device=q.device)
+    out = torch.empty((B, Lq, Hq, D), dtype=q.dtype, device=device)
+    lse = torch.empty((B, Hq, Lq), dtype=torch.float32, device=device)
     desc.out_batch, desc.out_token, desc.out_head = Lq * Hq * D, Hq * D, D
-    ws, n = _workspace(desc, 0, q.device)
-    _enqueue("trace_attention", q.device, C.byref(desc), q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(),
+    ws, n = _workspace(desc, 0, device)
+    _enqueue("trace_attention", device, C.byref(desc), q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(),
              lse.data_ptr(), _at(ws), n)
     return out, lse
 
@@ -127,10 +146,11 @@ def attention_backward(dout, q, k, v, out, lse, causal=False, query_start=None, 
     Gradients of shared key heads are summed over their query heads.  Queries that see no key and keys that no query sees get
     zero, whatever they (and dout) hold there."""
     _check("q", q, dims=4)
-    _check("dout", dout, like=q, dtype=q.dtype, shape=q.shape)
-    _check("out", out, like=q, dtype=q.dtype, shape=q.shape)
-    _check("lse", lse, like=q, dtype=torch.float32, shape=(q.shape[0], q.shape[2], q.shape[1]))
-    _need(lse.is_contiguous(), "lse must be contiguous")
+    _check("dout", dout, q.dtype, q.device, q.shape)
+    _check("out", out, q.dtype, q.device, q.shape)
+    _check("lse", lse, torch.float32, q.device, (q.shape[0], q.shape[2], q.shape[1]))
+    if not lse.is_contiguous():
+        _refuse("lse must be contiguous")
     desc = _attention_desc(q, k, v, causal, query_start, key_lengths, key_mask, scale, (out, dout))
     _gpu(q)
     dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v))
@@ -153,10 +173,14 @@ def rotary_frequencies(rot, base=10000.0, scaling="none", factor=1.0, trained_le
       "base"      the base raised by factor ** (rot / (rot - 2)): the slowest pair is stretched by the factor, the fastest not
       "by_turns"  pairs that make at least turns_kept turns over trained_length stay, those below turns_stretched are
                   divided by the factor, a linear ramp in between; scale = 1 + ln(factor) / 10 sharpens the scores"""
-    _need(isinstance(rot, int) and rot >= 2 and rot % 2 == 0, "rot %r must be even and positive", rot)
-    _need(scaling in ("none", "linear", "base", "by_turns"), "unknown scaling %r", scaling)
-    _need(base > 1 and factor >= 1, "base %g must be above 1 and factor %g at least 1", base, factor)
-    _need(scaling != "base" or rot > 2, "scaling by the base needs two pairs")
+    if not (isinstance(rot, int) and rot >= 2 and rot % 2 == 0):
+        _refuse("rot %r must be even and positive", rot)
+    if scaling not in ("none", "linear", "base", "by_turns"):
+        _refuse("unknown scaling %r", scaling)
+    if not (base > 1 and factor >= 1):
+        _refuse("base %g must be above 1 and factor %g at least 1", base, factor)
+    if scaling == "base" and rot == 2:
+        _refuse("scaling by the base needs two pairs")
     if scaling == "base":
         base = base * factor ** (rot / (rot - 2))
     f = float(base) ** (-2 * torch.arange(rot // 2, dtype=torch.float64) / rot)
@@ -164,8 +188,10 @@ def rotary_frequencies(rot, base=10000.0, scaling="none", factor=1.0, trained_le
     if scaling == "linear":
         f = f / factor
     elif scaling == "by_turns":
-        _need(trained_length is not None and trained_length >= 1, "scaling by turns needs the trained length")
-        _need(turns_kept > turns_stretched, "turns_kept %g must be above turns_stretched %g", turns_kept, turns_stretched)
+        if trained_length is None or trained_length < 1:
+            _refuse("scaling by turns needs the trained length")
+        if not turns_kept > turns_stretched:
+            _refuse("turns_kept %g must be above turns_stretched %g", turns_kept, turns_stretched)
         ramp = ((trained_length * f / (2 * math.pi) - turns_stretched) / (turns_kept - turns_stretched)).clamp(0, 1)
         f = f * ramp + f / factor * (1 - ramp)
         scale = 1 + 0.1 * math.log(factor)
@@ -179,24 +205,27 @@ def rotary(q, positions, freqs, k=None, interleaved=False, scale=1.0, inverse=Fa
     is also the gradient (of the same scale).  positions (L) or (B, L), int32 or int64, of any sign; freqs float64.
     inplace: the results replace q and k.  Returns the rotated q, or (q, k)."""
     _check("q", q, dims=4)
+    device = q.device
     B, L, Hq, D = q.shape
     if k is not None:
-        _check("k", k, like=q, dtype=q.dtype, dims=4)
-        _need(k.shape[0] == B and k.shape[1] == L and k.shape[3] == D, "k has shape %s, q %s", tuple(k.shape),
-              tuple(q.shape))
-    _check("freqs", freqs, like=q, dtype=torch.float64, dims=1)
+        _check("k", k, q.dtype, device, dims=4)
+        if k.shape[0] != B or k.shape[1] != L or k.shape[3] != D:
+            _refuse("k has shape %s, q %s", tuple(k.shape), tuple(q.shape))
+    _check("freqs", freqs, torch.float64, device, dims=1)
     rot = 2 * freqs.shape[0]
-    _need(2 <= rot <= D <= 1024, "%d rotated of %d head elements (at most 1024)", rot, D)
-    _need(isinstance(positions, torch.Tensor) and positions.dtype in (torch.int32, torch.int64),
-          "positions must be an int32 or int64 tensor")
-    _check("positions", positions, like=q, dtype=positions.dtype)
-    _need(tuple(positions.shape) in ((L,), (B, L)), "positions have shape %s, expected (%d,) or (%d, %d)",
-          tuple(positions.shape), L, B, L)
-    _need(math.isfinite(scale), "scale is not finite")
+    if not 2 <= rot <= D <= 1024:
+        _refuse("%d rotated of %d head elements (at most 1024)", rot, D)
+    if not (isinstance(positions, torch.Tensor) and positions.dtype in (torch.int32, torch.int64)):
+        _refuse("positions must be an int32 or int64 tensor")
+    _check("positions", positions, positions.dtype, device)
+    if positions.shape != (L,) and positions.shape != (B, L):
+        _refuse("positions have shape %s, expected (%d,) or (%d, %d)", tuple(positions.shape), L, B, L)
+    if not math.isfinite(scale):
+        _refuse("scale is not finite")
     if inplace:
         for name, t in (("q", q), ("k", k)):
-            _need(t is None or all(s != 0 or n <= 1 for s, n in zip(t.stride(), t.shape)),
-                  "%s is broadcast: it cannot be rotated in place", name)
+            if t is not None and any(s == 0 and n > 1 for s, n in zip(t.stride(), t.shape)):
+                _refuse("%s is broadcast: it cannot be rotated in place", name)
     _gpu(q)
     oq = q if inplace else torch.empty(q.shape, dtype=q.dtype, device=q.device)
     ok = k if k is None or inplace else torch.empty(k.shape, dtype=k.dtype, device=k.device)
@@ -213,55 +242,63 @@ def rotary(q, positions, freqs, k=None, interleaved=False, scale=1.0, inverse=Fa
 
 # ---------------------------------------------------------------------------------------------- norms ----
 
-def _rows(name, t):
-    """t (..., C) as (rows, C) without a copy."""
+def _row_stride(name, t):
+    """The distance of the rows of t (..., C)."""
+    if t.is_contiguous():
+        return t.shape[-1]
     try:
-        return t.view(-1, t.shape[-1]) if t.shape[-1] else t.new_empty(0, 0)
+        return t.view(-1, t.shape[-1]).stride(0)
     except RuntimeError:
-        raise ValueError("%s: the rows of a tensor with strides %s are not evenly spaced" % (name, t.stride()))
+        _refuse("%s: the rows of a tensor with strides %s are not evenly spaced", name, t.stride())
 
 
-def _table(name, t, like, groups, C):
+def _table(name, t, device, groups, columns):
     """A parameter of (C), (1, C) or a row for each conditioning group: whether it has one for each."""
-    if t is None:
-        return False
-    _check(name, t, like=like, dtype=torch.float32)
-    _need(tuple(t.shape) in ((C,), (1, C), (groups, C)), "%s has shape %s, expected (%d,) or (%d, %d)", name,
-          tuple(t.shape), C, groups, C)
-    _need(t.is_contiguous(), "%s must be contiguous", name)
-    return t.dim() == 2 and groups > 1 and t.shape[0] == groups
+    _check(name, t, torch.float32, device)
+    s = t.shape
+    if s != (columns,) and s != (1, columns) and s != (groups, columns):
+        _refuse("%s has shape %s, expected (%d,) or (%d, %d)", name, tuple(s), columns, groups, columns)
+    if not t.is_contiguous():
+        _refuse("%s must be contiguous", name)
+    return len(s) == 2 and groups > 1 and s[0] == groups
 
 
 def _norm_desc(x, y, gate, post_weight, weight, bias, kind, residual_scale, eps, rows_per_cond):
     _check("x", x)
-    _need(x.dim() >= 1 and 1 <= x.shape[-1] <= 16384, "x has shape %s (1..16384 columns)", tuple(x.shape))
-    C_ = x.shape[-1]
-    xr, yr = _rows("x", x), None
+    shape, device = x.shape, x.device
+    if not shape or not 1 <= shape[-1] <= 16384:
+        _refuse("x has shape %s (1..16384 columns)", tuple(shape))
+    columns = shape[-1]
+    rows = x.numel() // columns
+    if rows >= 1 << 31:
+        _refuse("more than 2^31 rows")
+    code = stream = _DTYPES[x.dtype]
+    ys = 0
     if y is not None:
-        _check("y", y, like=x, shape=x.shape)
-        _need(x.dtype in (torch.float32, y.dtype), "x is %s beside a block output of %s (float32, or the same)", x.dtype,
-              y.dtype)
-        yr = _rows("y", y)
-    else:
-        _need(gate is None and post_weight is None, "gate and post_weight belong to a block output y")
-    R = xr.shape[0]
-    _need(R < 1 << 31, "more than 2^31 rows")
-    _need(kind in _NORMS, "unknown norm %r", kind)
-    _need(math.isfinite(eps) and eps >= 0 and math.isfinite(residual_scale),
-          "eps %g and residual_scale %g must be finite, eps not negative", eps, residual_scale)
-    _need(rows_per_cond is None or (isinstance(rows_per_cond, int) and rows_per_cond >= 1),
-          "rows_per_cond %r must be a positive number", rows_per_cond)
-    rpc = min(rows_per_cond or max(R, 1), max(R, 1))
-    groups = -(-R // rpc) if R else 1
-    gate_cond = _table("gate", gate, x, groups, C_)
-    _need(not _table("post_weight", post_weight, x, 1, C_), "post_weight has one row")
-    w_cond, b_cond = _table("weight", weight, x, groups, C_), _table("bias", bias, x, groups, C_)
-    _need(weight is None or bias is None or w_cond == b_cond, "weight and bias must both have a row for each group, or "
-          "neither")
-    out = y if y is not None else x
-    return _cabi.NormDesc(_DTYPES[out.dtype], _DTYPES[x.dtype], R, C_, rpc, 1 if w_cond or b_cond else 0,
-                          1 if gate_cond else 0, _NORMS[kind], residual_scale, eps, xr.stride(0),
-                          0 if y is None else yr.stride(0), 0, 0)
+        _check("y", y, None, device, shape)
+        code = _DTYPES[y.dtype]
+        if stream and stream != code:
+            _refuse("x is %s beside a block output of %s (float32, or the same)", x.dtype, y.dtype)
+        ys = _row_stride("y", y)
+    elif gate is not None or post_weight is not None:
+        _refuse("gate and post_weight belong to a block output y")
+    if kind not in _NORMS:
+        _refuse("unknown norm %r", kind)
+    if not (math.isfinite(eps) and eps >= 0 and math.isfinite(residual_scale)):
+        _refuse("eps %g and residual_scale %g must be finite, eps not negative", eps, residual_scale)
+    if rows_per_cond is not None and not (isinstance(rows_per_cond, int) and rows_per_cond >= 1):
+        _refuse("rows_per_cond %r must be a positive number", rows_per_cond)
+    per = min(rows_per_cond or max(rows, 1), max(rows, 1))
+    groups = -(-rows // per) if rows else 1
+    gate_cond = gate is not None and _table("gate", gate, device, groups, columns)
+    if post_weight is not None and (_table("post_weight", post_weight, device, 1, columns)):
+        _refuse("post_weight has one row")
+    w_cond = weight is not None and _table("weight", weight, device, groups, columns)
+    b_cond = bias is not None and _table("bias", bias, device, groups, columns)
+    if weight is not None and bias is not None and w_cond != b_cond:
+        _refuse("weight and bias must both have a row for each group, or neither")
+    return _cabi.NormDesc(code, stream, rows, columns, per, 1 if w_cond or b_cond else 0, 1 if gate_cond else 0,
+                          _NORMS[kind], residual_scale, eps, _row_stride("x", x), ys, 0, 0)
 
 
 def residual_norm(x, y=None, gate=None, post_weight=None, weight=None, bias=None, kind="rms", residual_scale=1.0,
@@ -273,12 +310,16 @@ def residual_norm(x, y=None, gate=None, post_weight=None, weight=None, bias=None
     rows_per_cond consecutive rows of x: the scale, shift and gate that a conditioning gives to each trajectory.
     x, the residual stream, has y's type or fp32.  Returns (h, z); h is x where y is None, z None where norm is False."""
     desc = _norm_desc(x, y, gate, post_weight, weight, bias, kind, residual_scale, eps, rows_per_cond)
-    _need(norm or y is not None, "nothing to compute: no block output and no norm")
-    _need(norm or (weight is None and bias is None), "weight and bias belong to the norm")
+    if not norm:
+        if y is None:
+            _refuse("nothing to compute: no block output and no norm")
+        if weight is not None or bias is not None:
+            _refuse("weight and bias belong to the norm")
     _gpu(x)
-    h = x if y is None else torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    z = torch.empty(x.shape, dtype=x.dtype if y is None else y.dtype, device=x.device) if norm else None
-    _enqueue("trace_residual_norm", x.device, C.byref(desc), x.data_ptr(), _at(y), _at(gate), _at(post_weight),
+    device = x.device
+    h = x if y is None else torch.empty(x.shape, dtype=x.dtype, device=device)
+    z = torch.empty(x.shape, dtype=x.dtype if y is None else y.dtype, device=device) if norm else None
+    _enqueue("trace_residual_norm", device, C.byref(desc), x.data_ptr(), _at(y), _at(gate), _at(post_weight),
              _at(weight), _at(bias), None if y is None else h.data_ptr(), _at(z))
     return h, z
 
@@ -289,13 +330,14 @@ def residual_norm_backward(dh, dz, x, y=None, gate=None, post_weight=None, weigh
     Returns a dict of dx, dy, dgate, dpost_weight, dweight and dbias; None for what the call does not have."""
     desc = _norm_desc(x, y, gate, post_weight, weight, bias, kind, residual_scale, eps, rows_per_cond)
     out = x if y is None else y
-    _need(dh is not None or dz is not None, "neither dh nor dz")
+    if dh is None and dz is None:
+        _refuse("neither dh nor dz")
     if dh is not None:
-        _check("dh", dh, like=x, dtype=x.dtype, shape=x.shape)
-        desc.dh_stride = _rows("dh", dh).stride(0)
+        _check("dh", dh, x.dtype, x.device, x.shape)
+        desc.dh_stride = _row_stride("dh", dh)
     if dz is not None:
-        _check("dz", dz, like=x, dtype=out.dtype, shape=x.shape)
-        desc.dz_stride = _rows("dz", dz).stride(0)
+        _check("dz", dz, out.dtype, x.device, x.shape)
+        desc.dz_stride = _row_stride("dz", dz)
     _gpu(x)
     new = torch.empty if desc.rows and dz is not None else torch.zeros
     got = {"dx": torch.empty(x.shape, dtype=x.dtype, device=x.device),
