@@ -138,6 +138,17 @@ __device__ __forceinline__ unsigned long long key_bits(const AttnArgs& a, int b,
   return __ballot(on);
 }
 
+// Whether this lane's key of result register r counts: bit 8 (r / 4) + r % 4 of the 32 keys' word for lanes 0 .. 31, four
+// further for the others.  The word is uniform, so this is scalar work and one select a register.
+__device__ __forceinline__ bool key_on(unsigned word, int r) {
+  const int key = 8 * (r / 4) + r % 4;
+  const int low = (int)(word << (31 - key)) >> 31, high = (int)(word << (27 - key)) >> 31;
+  return __builtin_amdgcn_inverse_ballot_w64(((unsigned long long)(unsigned)high << 32) | (unsigned)low);
+}
+__device__ __forceinline__ unsigned word_of(unsigned long long bits, int t) {
+  return __builtin_amdgcn_readfirstlane((unsigned)(bits >> (32 * t)));
+}
+
 __device__ __forceinline__ int key_limit(const AttnArgs& a, int b) {
   if (!a.key_lengths) return a.Lk;
   const int n = a.key_lengths[b];
@@ -234,16 +245,21 @@ __global__ __launch_bounds__(NW * 64, sizeof(T) == 2 ? 2 : DP <= 64 ? 3 : 1) voi
     for (int t = 0; t < KT / 32; ++t)
 #pragma unroll
       for (int c = 0; c < NC; ++c) s[t] = Elem<T>::mma32(frag_at<T>(kt, TileR<T, DP>::frag(t * 32 + col, c, half)), qf[c], s[t]);
-    if (here != FULL || key0 + KT - 1 > sees - col) {     // sees - col: what the wave's first query sees
-      const unsigned long long mine = here >> (4 * half);
+    if (here != FULL) {
+#pragma unroll
+      for (int t = 0; t < KT / 32; ++t) {
+        const unsigned word = word_of(here, t);
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s[t][r] = key_on(word, r) ? s[t][r] : -INFINITY;
+      }
+    }
+    if (a.causal && key0 + KT - 1 > sees - col) {          // sees - col: what the wave's first query sees
       const int room = (int)max(-64L, min(64L, sees - key0)) - 4 * half;
 #pragma unroll
       for (int t = 0; t < KT / 32; ++t)
 #pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          const int key = t * 32 + 8 * (r / 4) + r % 4;
-          if (!((mine >> key) & 1) || key > room) s[t][r] = -INFINITY;
-        }
+        for (int r = 0; r < 16; ++r)
+          if (t * 32 + 8 * (r / 4) + r % 4 > room) s[t][r] = -INFINITY;
     }
     float top = -INFINITY;
 #pragma unroll
@@ -367,14 +383,16 @@ __global__ __launch_bounds__(64) void attn_few_kernel(AttnArgs a) {
       fetch(key0 + KT, bits);
     }
     if (here == 0u) continue;
-    if (here != ~0u || key0 + KT - 1 > start) {              // start: what query 0 sees
-      const unsigned mine = here >> (4 * half);
+    if (here != ~0u) {
+      const unsigned word = word_of(here, 0);
+#pragma unroll
+      for (int r = 0; r < 16; ++r) s[r] = key_on(word, r) ? s[r] : -INFINITY;
+    }
+    if (a.causal && key0 + KT - 1 > start) {                // start: what query 0 sees
       const int room = (int)max(-64L, min(64L, sees - key0)) - 4 * half;
 #pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        const int key = 8 * (r / 4) + r % 4;
-        if (!((mine >> key) & 1) || key > room) s[r] = -INFINITY;
-      }
+      for (int r = 0; r < 16; ++r)
+        if (8 * (r / 4) + r % 4 > room) s[r] = -INFINITY;
     }
     float top = s[0];
 #pragma unroll
@@ -562,7 +580,7 @@ __global__ __launch_bounds__(NW * 64, sizeof(T) == 2 ? 2 : DP <= 64 ? 3 : 1) voi
     __syncthreads();
     stage(key0, here);
     __syncthreads();
-    const bool partial = here != FULL || key0 + KT - 1 > sees - col;
+    const bool beyond = a.causal && key0 + KT - 1 > sees - col;
 #pragma unroll
     for (int t = 0; t < KT / 32; ++t) {
       f32x16 s = {}, dp = {};
@@ -572,14 +590,16 @@ __global__ __launch_bounds__(NW * 64, sizeof(T) == 2 ? 2 : DP <= 64 ? 3 : 1) voi
       for (int c = 0; c < NC; ++c) dp = Elem<T>::mma32(frag_at<T>(vt, TileR<T, DP>::frag(t * 32 + col, c, half)), gf[c], dp);
 #pragma unroll
       for (int r = 0; r < 16; ++r) s[r] = __builtin_amdgcn_exp2f(fmaf(s[r], a.scale_log2, -lse2)) * (dp[r] - delta);
-      if (partial) {
-        const unsigned long long mine = here >> (4 * half);
+      if (here != FULL) {
+        const unsigned word = word_of(here, t);
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s[r] = key_on(word, r) ? s[r] : 0.f;
+      }
+      if (beyond) {
         const int room = (int)max(-64L, min(64L, sees - key0)) - 4 * half;
 #pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          const int key = t * 32 + 8 * (r / 4) + r % 4;
-          if (!((mine >> key) & 1) || key > room) s[r] = 0.f;
-        }
+        for (int r = 0; r < 16; ++r)
+          if (t * 32 + 8 * (r / 4) + r % 4 > room) s[r] = 0.f;
       }
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
@@ -896,13 +916,12 @@ __global__ __launch_bounds__(QB * KB * 64, DP <= 64 ? 2 : 1) void attn_short_bac
     }
     delta += __shfl_xor(delta, 32, 64);
     {
-      const unsigned mine = (unsigned)(bits >> (ki * 32)) >> (4 * half);
+      const unsigned word = word_of(bits, ki);
       const int room = (int)max(-64L, min(64L, i + start - ki * 32)) - 4 * half;
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
-        const int key = 8 * (r / 4) + r % 4;
         const float p = __builtin_amdgcn_exp2f(fmaf(s[r], a.scale_log2, -lse2));
-        const bool on = ((mine >> key) & 1) && key <= room;
+        const bool on = key_on(word, r) && 8 * (r / 4) + r % 4 <= room;
         s[r] = on ? p : 0.f;
         dp[r] = on ? p * (dp[r] - delta) : 0.f;
       }
