@@ -130,6 +130,17 @@ __device__ __forceinline__ typename Elem<T>::V8 as_operand(const f32x16& s, int 
   return v;
 }
 
+// fp16: P and dS are rounded as 16 P and 16 dS.  A row of n keys holds P of about 1 / n, which from n = 2^14 on, and dS sooner,
+// would fall among fp16's subnormals.  16 dS overflows where |dS| passes 4094, and |dS| is at most half the largest |dout . v|.
+template <typename T>
+constexpr float P_SHIFT = 0.f;
+template <>
+inline constexpr float P_SHIFT<_Float16> = 4.f;
+template <typename T>
+constexpr float P_UNSHIFT = 1.f;
+template <>
+inline constexpr float P_UNSHIFT<_Float16> = 0.0625f;
+
 // One bit per key of the tile at key0: below the sequence's length and not masked.  The same in every wave.
 __device__ __forceinline__ unsigned long long key_bits(const AttnArgs& a, int b, int key0, int len) {
   const int key = key0 + (int)(threadIdx.x & 63);
@@ -522,7 +533,7 @@ __global__ __launch_bounds__(NW * 64, sizeof(T) == 2 ? 2 : DP <= 64 ? 3 : 1) voi
 
   const float lse = i < a.Lq ? a.lse_in[row] : -INFINITY;
   const bool live = lse != -INFINITY;                     // a row that sees nothing has no gradient, whatever it holds
-  const float lse2 = live ? lse * LOG2E : INFINITY;
+  const float lse2 = live ? fmaf(lse, LOG2E, -P_SHIFT<T>) : INFINITY;
   V8 qf[NC], gf[NC];
   float delta = 0.f;
 #pragma unroll
@@ -611,14 +622,15 @@ __global__ __launch_bounds__(NW * 64, sizeof(T) == 2 ? 2 : DP <= 64 ? 3 : 1) voi
     }
   }
   if (i >= a.Lq) return;
+  const float back = a.scale * P_UNSHIFT<T>;
   T* p = (T*)a.dq + b * a.vdq.sb + hq * a.vdq.sh + (long)i * a.vdq.sl;
 #pragma unroll
   for (int dt = 0; dt < ND; ++dt)
 #pragma unroll
     for (int g = 0; g < 4; ++g) {
       const int d = dt * 32 + g * 8 + half * 4;
-      const f32v4 w = {acc[dt][4 * g] * a.scale, acc[dt][4 * g + 1] * a.scale, acc[dt][4 * g + 2] * a.scale,
-                       acc[dt][4 * g + 3] * a.scale};
+      const f32v4 w = {acc[dt][4 * g] * back, acc[dt][4 * g + 1] * back, acc[dt][4 * g + 2] * back,
+                       acc[dt][4 * g + 3] * back};
       if (d < a.D) store4<T>(p + d, w, a.D - d, vec);
     }
 }
@@ -717,7 +729,7 @@ __global__ __launch_bounds__(NW * 64, sizeof(T) == 2 || DP <= 64 ? 2 : 1) void a
       const long at = ((long)b * a.Hq + hq) * a.Lq + q0 + tid;
       const float x = q0 + tid < a.Lq ? a.lse_in[at] : -INFINITY;
       const float y = q0 + tid < a.Lq ? a.delta[at] : 0.f;
-      lse2s[tid] = x == -INFINITY ? INFINITY : x * LOG2E;
+      lse2s[tid] = x == -INFINITY ? INFINITY : fmaf(x, LOG2E, -P_SHIFT<T>);
       deltas[tid] = x == -INFINITY ? 0.f : y;
     }
   };
@@ -790,6 +802,7 @@ __global__ __launch_bounds__(NW * 64, sizeof(T) == 2 || DP <= 64 ? 2 : 1) void a
       }
     return;
   }
+  const float back = a.scale * P_UNSHIFT<T>;
   T* pk = (T*)a.dk + b * a.vdk.sb + hk * a.vdk.sh + (long)j * a.vdk.sl;
   T* pv = (T*)a.dv + b * a.vdv.sb + hk * a.vdv.sh + (long)j * a.vdv.sl;
 #pragma unroll
@@ -798,9 +811,10 @@ __global__ __launch_bounds__(NW * 64, sizeof(T) == 2 || DP <= 64 ? 2 : 1) void a
     for (int g = 0; g < 4; ++g) {
       const int d = dt * 32 + g * 8 + half * 4;
       if (d >= a.D) continue;
-      const f32v4 w = {dk[dt][4 * g] * a.scale, dk[dt][4 * g + 1] * a.scale, dk[dt][4 * g + 2] * a.scale,
-                       dk[dt][4 * g + 3] * a.scale};
-      const f32v4 x = {dv[dt][4 * g], dv[dt][4 * g + 1], dv[dt][4 * g + 2], dv[dt][4 * g + 3]};
+      const f32v4 w = {dk[dt][4 * g] * back, dk[dt][4 * g + 1] * back, dk[dt][4 * g + 2] * back,
+                       dk[dt][4 * g + 3] * back};
+      const f32v4 x = {dv[dt][4 * g] * P_UNSHIFT<T>, dv[dt][4 * g + 1] * P_UNSHIFT<T>, dv[dt][4 * g + 2] * P_UNSHIFT<T>,
+                       dv[dt][4 * g + 3] * P_UNSHIFT<T>};
       store4<T>(pk + d, w, a.D - d, vec);
       store4<T>(pv + d, x, a.D - d, vec);
     }
@@ -870,13 +884,14 @@ __global__ __launch_bounds__(QB * KB * 64, DP <= 64 ? 2 : 1) void attn_short_bac
 #pragma unroll
     for (int e = 0; e < 4; ++e) *reinterpret_cast<V8*>(kt + (quad * 4 + e) * S + d) = t.r[e];
   }
+  const float back = a.scale * P_UNSHIFT<T>;
   f32x16 dk[KTILES] = {}, dv[KTILES] = {};
   for (int g = 0; g < a.G; ++g) {
     const int hq = hk * a.G + g;
     const float* lse_row = a.lse_in + ((long)b * a.Hq + hq) * a.Lq;
     const float lse = i < a.Lq ? lse_row[i] : -INFINITY;
     const bool live = lse != -INFINITY;                                  // else: no gradient, whatever the row holds
-    const float lse2 = live ? lse * LOG2E : INFINITY;
+    const float lse2 = live ? fmaf(lse, LOG2E, -P_SHIFT<T>) : INFINITY;
     V8 of[NC];
     {
       const T* p = (const T*)a.out_in + b * a.vo.sb + hq * a.vo.sh + (long)(live ? i : 0) * a.vo.sl;
@@ -972,7 +987,7 @@ __global__ __launch_bounds__(QB * KB * 64, DP <= 64 ? 2 : 1) void attn_short_bac
         for (int q = 0; q < 4; ++q) {
           const int d = t % ND * 32 + q * 8 + half * 4;
           if (row < a.Lq && d < a.D)
-            store4<T>(p + d, f32v4{dq[4 * q] * a.scale, dq[4 * q + 1] * a.scale, dq[4 * q + 2] * a.scale, dq[4 * q + 3] * a.scale},
+            store4<T>(p + d, f32v4{dq[4 * q] * back, dq[4 * q + 1] * back, dq[4 * q + 2] * back, dq[4 * q + 3] * back},
                       a.D - d, vec);
         }
       }
@@ -988,9 +1003,10 @@ __global__ __launch_bounds__(QB * KB * 64, DP <= 64 ? 2 : 1) void attn_short_bac
     for (int q = 0; q < 4; ++q) {
       const int d = t % ND * 32 + q * 8 + half * 4;
       if (d >= a.D) continue;
-      store4<T>(pk + d, f32v4{dk[n][4 * q] * a.scale, dk[n][4 * q + 1] * a.scale, dk[n][4 * q + 2] * a.scale, dk[n][4 * q + 3] * a.scale},
+      store4<T>(pk + d, f32v4{dk[n][4 * q] * back, dk[n][4 * q + 1] * back, dk[n][4 * q + 2] * back, dk[n][4 * q + 3] * back},
                 a.D - d, vec);
-      store4<T>(pv + d, f32v4{dv[n][4 * q], dv[n][4 * q + 1], dv[n][4 * q + 2], dv[n][4 * q + 3]}, a.D - d, vec);
+      store4<T>(pv + d, f32v4{dv[n][4 * q] * P_UNSHIFT<T>, dv[n][4 * q + 1] * P_UNSHIFT<T>, dv[n][4 * q + 2] * P_UNSHIFT<T>,
+                              dv[n][4 * q + 3] * P_UNSHIFT<T>}, a.D - d, vec);
     }
   }
 }
@@ -1014,7 +1030,10 @@ __global__ __launch_bounds__(256) void attn_sum_kernel(AttnArgs a) {
     }
   }
 #pragma unroll
-  for (int e = 0; e < 4; ++e) dk[e] *= a.scale;
+  for (int e = 0; e < 4; ++e) {
+    dk[e] *= a.scale * P_UNSHIFT<T>;
+    dv[e] *= P_UNSHIFT<T>;
+  }
   const int j = (int)(row % a.Lk), hk = (int)(row / a.Lk % a.Hk), b = (int)(row / a.Lk / a.Hk);
   store4<T>((T*)a.dk + b * a.vdk.sb + hk * a.vdk.sh + (long)j * a.vdk.sl + d, dk, a.D - d, a.vec);
   store4<T>((T*)a.dv + b * a.vdv.sb + hk * a.vdv.sh + (long)j * a.vdv.sl + d, dv, a.D - d, a.vec);
