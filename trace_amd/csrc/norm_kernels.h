@@ -63,6 +63,12 @@ __device__ __forceinline__ float team_sum(float v, float* red, int& turn) {
   return t;
 }
 
+// The team's number in the workgroup, in a scalar register: a row's addresses are then a uniform base and a lane's offset.
+template <int TPR>
+__device__ __forceinline__ int team_of() {
+  return TPR == 64 ? __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) : 0;
+}
+
 template <int TPR, int V, int K>
 struct RowStats {
   float mean, rstd;
@@ -95,7 +101,7 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void residual_norm_kernel(No
   constexpr int NT = TPR < 256 ? 256 : TPR;
   __shared__ float red[2 * (NT / 64)];
   const int lane = threadIdx.x % TPR;
-  const long row = (long)blockIdx.x * (NT / TPR) + threadIdx.x / TPR;
+  const long row = (long)blockIdx.x * (NT / TPR) + team_of<TPR>();
   if (row >= a.R) return;                                     // TPR > 64: a workgroup is one team
   int turn = 0;
   const int g = (int)(row / a.rpc);
@@ -165,7 +171,7 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void residual_norm_backward_
   __shared__ float red[2 * (NT / 64)];
   __shared__ float comb[TEAMS > 1 ? (TEAMS - 1) * TPR * V * K : 1];
   const int lane = threadIdx.x % TPR;
-  const int team = blockIdx.x * TEAMS + threadIdx.x / TPR;
+  const int team = blockIdx.x * TEAMS + team_of<TPR>();
   int turn = 0;
   float sg[K][V] = {}, sw[K][V] = {}, sb[K][V] = {}, sp[K][V] = {};
   const long first = (long)team * a.per_team;
