@@ -846,8 +846,27 @@ __device__ __forceinline__ typename Elem<T>::V8 frag_rows(const T* p, int stride
   return v;
 }
 
+// acc += sum over c < N of mma32(A(c), B(c)), the operands of step c + 1 read from LDS while step c runs: left to itself the
+// compiler waits for every read right before its use, which idles the matrix pipe for half of an LDS latency each time.
+template <typename T, int N, typename FA, typename FB>
+__device__ __forceinline__ void mma_ahead(f32x16& acc, FA fa, FB fb) {
+  typename Elem<T>::V8 x[2], y[2];
+  x[0] = fa(0);
+  y[0] = fb(0);
+#pragma unroll
+  for (int c = 0; c < N; ++c) {
+    if (c + 1 < N) {
+      x[(c + 1) & 1] = fa(c + 1);
+      y[(c + 1) & 1] = fb(c + 1);
+    }
+    __builtin_amdgcn_sched_barrier(0);
+    acc = Elem<T>::mma32(x[c & 1], y[c & 1], acc);
+    __builtin_amdgcn_sched_barrier(0);
+  }
+}
+
 template <typename T, int DP, int QB, int KB>
-__global__ __launch_bounds__(QB * KB * 64, DP <= 64 ? 2 : 1) void attn_short_backward_kernel(AttnArgs a) {
+__global__ __launch_bounds__(QB * KB * 64, DP == 32 || (DP == 64 && QB * KB == 4) ? 2 : 1) void attn_short_backward_kernel(AttnArgs a) {
   typedef typename Elem<T>::V8 V8;
   constexpr int NW = QB * KB, NT = NW * 64, NC = DP / 16, ND = DP / 32, S = TileN<T, DP>::S, XS = TileN<T, 32 * KB>::S;
   constexpr int UQ = 8 * QB * (DP / 8), UK = 8 * KB * (DP / 8);          // staging units of a query / key tile
@@ -869,67 +888,89 @@ __global__ __launch_bounds__(QB * KB * 64, DP <= 64 ? 2 : 1) void attn_short_bac
   const int i = qi * 32 + col;                                           // this lane's query
   const T* kb = (const T*)a.k + b * a.vk.sb + hk * a.vk.sh;
   const T* vb = (const T*)a.v + b * a.vv.sb + hk * a.vv.sh;
+  // All loads of a head are under way before the first is waited for, and none hangs on another's result: rows that do not
+  // exist are read from the last one that does, and what must not count is made zero on its way to LDS.
+  constexpr int UKT = (UK + NT - 1) / NT, UQT = (2 * UQ + NT - 1) / NT;
   V8 vf[NC];
+  Unit<T> ku[UKT];
   {
     const int j = ki * 32 + col;
-    const bool on = (bits >> j) & 1;
-    const T* p = vb + (long)(on ? j : 0) * a.vv.sl;
+    const T* p = vb + (long)min(j, a.Lk - 1) * a.vv.sl;
 #pragma unroll
-    for (int c = 0; c < NC; ++c) vf[c] = load8<T>(p + c * 16 + half * 8, on ? a.D - c * 16 - half * 8 : 0, vec);
-  }
-  for (int u = tid; u < UK; u += NT) {
-    const int quad = u / (DP / 8), d = u % (DP / 8) * 8;
-    Unit<T> t;
-    t.load(kb, a.vk.sl, quad * 4, a.Lk, d, a.D, (unsigned)(bits >> (quad * 4)) & 15u, vec, whole_d && 32 * KB <= len && !a.key_mask);
+    for (int c = 0; c < NC; ++c) vf[c] = load8<T>(p + c * 16 + half * 8, a.D - c * 16 - half * 8, vec);
 #pragma unroll
-    for (int e = 0; e < 4; ++e) *reinterpret_cast<V8*>(kt + (quad * 4 + e) * S + d) = t.r[e];
+    for (int n = 0; n < UKT; ++n) {
+      const int u = min(tid + n * NT, UK - 1), quad = u / (DP / 8), d = u % (DP / 8) * 8;
+      ku[n].load(kb, a.vk.sl, quad * 4, a.Lk, d, a.D, 15u, vec, whole_d && 32 * KB <= a.Lk);
+    }
   }
-  const float back = a.scale * P_UNSHIFT<T>;
   f32x16 dk[KTILES] = {}, dv[KTILES] = {};
+  const float back = a.scale * P_UNSHIFT<T>;
   for (int g = 0; g < a.G; ++g) {
     const int hq = hk * a.G + g;
     const float* lse_row = a.lse_in + ((long)b * a.Hq + hq) * a.Lq;
-    const float lse = i < a.Lq ? lse_row[i] : -INFINITY;
-    const bool live = lse != -INFINITY;                                  // else: no gradient, whatever the row holds
-    const float lse2 = live ? fmaf(lse, LOG2E, -P_SHIFT<T>) : INFINITY;
     V8 of[NC];
+    Unit<T> un[UQT];
+    float seen[UQT][4];
+    const float lse_i = lse_row[min(i, a.Lq - 1)];
     {
-      const T* p = (const T*)a.out_in + b * a.vo.sb + hq * a.vo.sh + (long)(live ? i : 0) * a.vo.sl;
+      const T* p = (const T*)a.out_in + b * a.vo.sb + hq * a.vo.sh + (long)min(i, a.Lq - 1) * a.vo.sl;
 #pragma unroll
-      for (int c = 0; c < NC; ++c) of[c] = load8<T>(p + c * 16 + half * 8, live ? a.D - c * 16 - half * 8 : 0, vec);
+      for (int c = 0; c < NC; ++c) of[c] = load8<T>(p + c * 16 + half * 8, a.D - c * 16 - half * 8, vec);
     }
-    if (g > 0) __syncthreads();                                          // the last head's tiles are done with
-    for (int u = tid; u < 2 * UQ; u += NT) {
+#pragma unroll
+    for (int n = 0; n < UQT; ++n) {
+      const int u = min(tid + n * NT, 2 * UQ - 1);
       const bool is_g = u >= UQ;
       const int w = is_g ? u - UQ : u, quad = w / (DP / 8), d = w % (DP / 8) * 8;
-      unsigned ok = 0;
-      float seen[4];
-#pragma unroll
-      for (int e = 0; e < 4; ++e) seen[e] = quad * 4 + e < a.Lq ? lse_row[quad * 4 + e] : -INFINITY;
-      const long sl = is_g ? a.vdo.sl : a.vq.sl;
       const T* base = is_g ? (const T*)a.dout + b * a.vdo.sb + hq * a.vdo.sh : (const T*)a.q + b * a.vq.sb + hq * a.vq.sh;
-      Unit<T> t;
-      const int left = a.Lq - quad * 4;
-      ok = left >= 4 ? 15u : left > 0 ? (1u << left) - 1 : 0u;
-      t.load(base, sl, quad * 4, a.Lq, d, a.D, ok, vec, whole_d && 32 * QB <= a.Lq);
+      un[n].load(base, is_g ? a.vdo.sl : a.vq.sl, quad * 4, a.Lq, d, a.D, 15u, vec, whole_d && 32 * QB <= a.Lq);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) seen[n][e] = lse_row[min(quad * 4 + e, a.Lq - 1)];
+    }
+    if (g > 0) {
+      __syncthreads();                                                   // the last head's tiles are done with
+    } else {
+#pragma unroll
+      for (int n = 0; n < UKT; ++n) {
+        const int u = tid + n * NT, quad = u / (DP / 8), d = u % (DP / 8) * 8;
+        if (u >= UK) continue;
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          *reinterpret_cast<V8*>(kt + (quad * 4 + e) * S + d) = (bits >> (quad * 4 + e)) & 1 ? ku[n].r[e] : V8{};
+      }
+      if (!((bits >> (ki * 32 + col)) & 1)) {
+#pragma unroll
+        for (int c = 0; c < NC; ++c) vf[c] = V8{};
+      }
+    }
+    // queries that see nothing, and those past the end, count as absent, whatever they hold
+    const bool live = i < a.Lq && lse_i != -INFINITY;
+    const float lse2 = live ? fmaf(lse_i, LOG2E, -P_SHIFT<T>) : INFINITY;
+#pragma unroll
+    for (int n = 0; n < UQT; ++n) {
+      const int u = tid + n * NT;
+      const bool is_g = u >= UQ;
+      const int w = is_g ? u - UQ : u, quad = w / (DP / 8), d = w % (DP / 8) * 8;
+      if (u >= 2 * UQ) continue;
       T* to = (is_g ? gt : qt) + quad * 4 * S + d;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) *reinterpret_cast<V8*>(to + e * S) = seen[e] == -INFINITY ? V8{} : t.r[e];
+      for (int e = 0; e < 4; ++e)
+        *reinterpret_cast<V8*>(to + e * S) = quad * 4 + e < a.Lq && seen[n][e] != -INFINITY ? un[n].r[e] : V8{};
     }
     __syncthreads();
     f32x16 s = {}, dp = {};
     float delta = 0.f;
-#pragma unroll
-    for (int c = 0; c < NC; ++c) {
-      const int at = c * 16 + half * 8;
-      s = Elem<T>::mma32(*reinterpret_cast<const V8*>(kt + (ki * 32 + col) * S + at),
-                         *reinterpret_cast<const V8*>(qt + i * S + at), s);
-      const V8 gf = *reinterpret_cast<const V8*>(gt + i * S + at);
-      dp = Elem<T>::mma32(vf[c], gf, dp);
+    mma_ahead<T, NC>(s, [&](int c) { return *reinterpret_cast<const V8*>(kt + (ki * 32 + col) * S + c * 16 + half * 8); },
+                     [&](int c) { return *reinterpret_cast<const V8*>(qt + i * S + c * 16 + half * 8); });
+    mma_ahead<T, NC>(dp, [&](int c) { return vf[c]; }, [&](int c) {
+      const V8 gf = *reinterpret_cast<const V8*>(gt + i * S + c * 16 + half * 8);
 #pragma unroll
       for (int j = 0; j < 8; ++j) delta = fmaf((float)gf[j], (float)of[c][j], delta);
-    }
+      return gf;
+    });
     delta += __shfl_xor(delta, 32, 64);
+    delta = live ? delta : 0.f;
     {
       const unsigned word = word_of(bits, ki);
       const int room = (int)max(-64L, min(64L, i + start - ki * 32)) - 4 * half;
@@ -953,10 +994,8 @@ __global__ __launch_bounds__(QB * KB * 64, DP <= 64 ? 2 : 1) void attn_short_bac
     for (int n = 0; n < KTILES; ++n) {
       const int t = wave + n * NW;
       if (KB * ND % NW == 0 || t < KB * ND) {
-#pragma unroll
-        for (int c = 0; c < 2 * QB; ++c)
-          dv[n] = Elem<T>::mma32(frag_rows<T>(gt + c * 16 * S + t % ND * 32 + col, S, half),
-                                 frag_rows<T>(xt + c * 16 * XS + t / ND * 32 + col, XS, half), dv[n]);
+        mma_ahead<T, 2 * QB>(dv[n], [&](int c) { return frag_rows<T>(gt + c * 16 * S + t % ND * 32 + col, S, half); },
+                             [&](int c) { return frag_rows<T>(xt + c * 16 * XS + t / ND * 32 + col, XS, half); });
       }
     }
     __syncthreads();
@@ -966,10 +1005,8 @@ __global__ __launch_bounds__(QB * KB * 64, DP <= 64 ? 2 : 1) void attn_short_bac
     for (int n = 0; n < KTILES; ++n) {
       const int t = wave + n * NW;
       if (KB * ND % NW == 0 || t < KB * ND) {
-#pragma unroll
-        for (int c = 0; c < 2 * QB; ++c)
-          dk[n] = Elem<T>::mma32(frag_rows<T>(qt + c * 16 * S + t % ND * 32 + col, S, half),
-                                 frag_rows<T>(xt + c * 16 * XS + t / ND * 32 + col, XS, half), dk[n]);
+        mma_ahead<T, 2 * QB>(dk[n], [&](int c) { return frag_rows<T>(qt + c * 16 * S + t % ND * 32 + col, S, half); },
+                             [&](int c) { return frag_rows<T>(xt + c * 16 * XS + t / ND * 32 + col, XS, half); });
       }
     }
 #pragma unroll
@@ -977,10 +1014,8 @@ __global__ __launch_bounds__(QB * KB * 64, DP <= 64 ? 2 : 1) void attn_short_bac
       const int t = wave + n * NW;
       if (QB * ND % NW == 0 || t < QB * ND) {
         f32x16 dq = {};
-#pragma unroll
-        for (int c = 0; c < 2 * KB; ++c)
-          dq = Elem<T>::mma32(frag_rows<T>(kt + c * 16 * S + t % ND * 32 + col, S, half),
-                              frag_slots<T>(xt + (t / ND * 32 + col) * XS + c * 16, half), dq);
+        mma_ahead<T, 2 * KB>(dq, [&](int c) { return frag_rows<T>(kt + c * 16 * S + t % ND * 32 + col, S, half); },
+                             [&](int c) { return frag_slots<T>(xt + (t / ND * 32 + col) * XS + c * 16, half); });
         const int row = t / ND * 32 + col;
         T* p = (T*)a.dq + b * a.vdq.sb + hq * a.vdq.sh + (long)row * a.vdq.sl;
 #pragma unroll
