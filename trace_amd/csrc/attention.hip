@@ -49,7 +49,8 @@ AttnArgs common_args(const trace_attention_desc& d) {
 
 int padded_dim(int D) { return D <= 32 ? 32 : D <= 64 ? 64 : 128; }
 
-// The form for few queries.  waves: enough to keep every CU's memory queue full (8 a CU measured best); a range has at
+// The form for few queries.  Ranges: one wave a SIMD, which is what the registers of the kernel leave room for (1024 and 2048 waves
+// measured alike, 1536 and 4096 a fifth slower: a second, partly filled round); a range has at
 // least 64 keys.
 struct FewPlan {
   bool use;
@@ -61,7 +62,7 @@ FewPlan few_plan(const trace_attention_desc& d) {
   const int64_t N = (int64_t)d.Lq * G, tiles = (N + 31) / 32, pairs = (int64_t)d.B * d.Hk;
   FewPlan p{};
   p.use = d.Lq <= 16;
-  int64_t splits = (2048 + pairs * tiles - 1) / (pairs * tiles);
+  int64_t splits = (1024 + pairs * tiles - 1) / (pairs * tiles);
   const int64_t most = (d.Lk + 63) / 64;
   splits = splits < most ? splits : most;
   p.splits = (int)(splits < 1 ? 1 : splits < ATTN_MAX_SPLITS ? splits : ATTN_MAX_SPLITS);

@@ -493,9 +493,10 @@ __global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a) {
   __syncthreads();
   const int d = tid % DP, g = tid / DP;
   float t = 0.f;
-  for (int s = g; s < a.splits; s += GR) {
-    const float w = weight[s];
-    if (w >= 0.f || w != w) t = fmaf(w, a.part_o[(row * a.splits + s) * DP + d], t);
+#pragma unroll 8
+  for (int s = g; s < a.splits; s += GR) {                  // loads without a branch, so that eight are under way at a time
+    const float w = weight[s], x = a.part_o[(row * a.splits + s) * DP + d];
+    t += w >= 0.f || w != w ? w * x : 0.f;
   }
   sums[tid] = t;
   __syncthreads();
