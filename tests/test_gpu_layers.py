@@ -187,6 +187,28 @@ def test_attention_passes_nan_on_where_it_is_seen():
 
 
 @pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("Lq, Lk", [(3, 40), (40, 60), (70, 300), (140, 200)])
+def test_attention_ignores_what_lies_past_the_last_query(dtype, Lq, Lk):
+    """A cache with room behind the positions that causality lets any query see."""
+    q, k, v = inputs(dtype, 2, Lq, Lk, 4, 2, 64)
+    start = torch.tensor([Lk - Lq - 9, -2], dtype=torch.int32, device=DEV)
+    want = compare(q, k, v, causal=True, query_start=start)
+    for b in range(2):
+        k[b, max(0, int(start[b]) + Lq):] = math.nan
+        v[b, max(0, int(start[b]) + Lq):] = math.inf
+    got = compare(q, k, v, causal=True, query_start=start)
+    for a, b in zip(want, got):
+        assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("size", [(300, 70, 70, 4, 2, 32), (600, 3, 40, 4, 2, 16), (150, 100, 90, 4, 4, 64), (40, 129, 200, 8, 8, 128)])
+def test_attention_of_many_heads(dtype, size):
+    """Enough workgroups that no kernel's loop is cut into shares."""
+    compare(*inputs(dtype, *size), causal=True)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("spread", [30.0, 300.0])
 def test_attention_of_peaked_scores(dtype, spread):
     """Scores far apart: one key carries a row, the exponentials of the others vanish; the running maximum grows late."""
@@ -374,6 +396,17 @@ def test_rotary_in_place_in_windows_of_a_projection(dtype):
         assert torch.equal(qkv[:, :, :H], want[0]) and torch.equal(qkv[:, :, H:2 * H], want[1])
         assert torch.equal(qkv[:, :, 2 * H:], before[:, :, 2 * H:])
         assert torch.equal(want[0][..., 16:], before[:, :, :H, 16:])
+
+
+def test_rotary_in_place_beside_each_other_in_a_head():
+    """q and k as the two halves of every head's row: windows of one layout that do not overlap."""
+    g = torch.Generator(DEV).manual_seed(6)
+    room = torch.randn(2, 5, 3, 2, 16, generator=g, device=DEV)
+    q, k = room[:, :, :, 0], room[:, :, :, 1]
+    freqs, _ = layers.rotary_frequencies(16, device=DEV)
+    want = layers.rotary(q, torch.arange(5, device=DEV), freqs, k=k)
+    layers.rotary(q, torch.arange(5, device=DEV), freqs, k=k, inplace=True)
+    assert torch.equal(q, want[0]) and torch.equal(k, want[1])
 
 
 def test_rotary_gradient_is_the_transpose():
@@ -577,6 +610,14 @@ def test_residual_norm_of_extreme_rows():
     x[3, 100] = math.nan
     _, z = layers.residual_norm(x, kind="layer")
     assert bool(torch.isnan(z[3]).all()) and bool(torch.isfinite(z[[0, 1, 2, 4, 5]]).all())
+
+
+def test_residual_norm_of_more_rows_than_one_launch_holds():
+    """2^23 rows of one column go out in a launch."""
+    x = torch.randn(2 ** 23 + 5, 1, device=DEV, generator=torch.Generator(DEV).manual_seed(1))
+    _, z = layers.residual_norm(x, kind="rms")
+    want = x.double() / torch.sqrt(x.double() ** 2 + 1e-5)
+    near(z, want, 8 * F * want.abs(), "z")
 
 
 def test_residual_norm_of_nothing():

@@ -81,6 +81,8 @@ def test_attention_backward_refuses_results_of_another_call():
     (lambda a: a.update(positions=torch.zeros(3, 3, dtype=torch.int64)), "shape"),
     (lambda a: a.update(scale=float("inf")), "finite"),
     (lambda a: a.update(k=a["k"][:, :, :1].expand(2, 3, 2, 16), inplace=True), "broadcast"),
+    (lambda a: a.update(k=a["q"], inplace=True), "share memory"),
+    (lambda a: a.update(k=a["q"][:, :, 2:], inplace=True), "share memory"),
 ])
 def test_rotary_refuses(change, text):
     a = dict(q=torch.zeros(2, 3, 4, 16), k=torch.zeros(2, 3, 2, 16), positions=torch.arange(3),

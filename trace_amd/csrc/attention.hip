@@ -47,50 +47,63 @@ AttnArgs common_args(const trace_attention_desc& d) {
   return a;
 }
 
+// Waves of a workgroup over `rows` tokens: as many as there are 32-row tiles, up to four.
+int waves_for(int rows) { return rows <= 32 ? 1 : rows <= 64 ? 2 : 4; }
+int64_t items_of(int rows, int64_t heads) { return (rows + 32 * waves_for(rows) - 1) / (32 * waves_for(rows)) * heads; }
+
 int padded_dim(int D) { return D <= 32 ? 32 : D <= 64 ? 64 : 128; }
 
-// The form for few queries.  Ranges: one wave a SIMD, which is what the registers of the kernel leave room for (1024 and 2048 waves
-// measured alike, 1536 and 4096 a fifth slower: a second, partly filled round); a range has at
-// least 64 keys.
-struct FewPlan {
-  bool use;
+// Into how many shares the loop of a kernel with `items` workgroups is cut for `target` of them: at most 16, and `most`.
+int shares(int64_t items, int64_t most, int target) {
+  int64_t n = items > 0 ? (target + items - 1) / items : 1;
+  n = n < most ? n : most;
+  return (int)(n < 1 ? 1 : n < 16 ? n : 16);
+}
+
+// The forward pass.  Up to 16 queries the heads of a group share a tile (attn_few_kernel), with one wave a SIMD, which is what the
+// registers of that kernel leave room for (1024 and 2048 waves measured alike, 1536 and 4096 a fifth slower: a second, partly filled
+// round), in ranges of at least 64 keys.  Otherwise two workgroups a CU, in ranges of at least two tiles.
+struct ForwardPlan {
+  bool few;
   int splits;
-  int64_t rows, ml_bytes, bytes;     // bytes of workspace
+  int64_t ml_bytes, bytes;           // of workspace
 };
-FewPlan few_plan(const trace_attention_desc& d) {
-  const int G = d.Hq / d.Hk;
-  const int64_t N = (int64_t)d.Lq * G, tiles = (N + 31) / 32, pairs = (int64_t)d.B * d.Hk;
-  FewPlan p{};
-  p.use = d.Lq <= 16;
-  int64_t splits = (1024 + pairs * tiles - 1) / (pairs * tiles);
-  const int64_t most = (d.Lk + 63) / 64;
-  splits = splits < most ? splits : most;
-  p.splits = (int)(splits < 1 ? 1 : splits < ATTN_MAX_SPLITS ? splits : ATTN_MAX_SPLITS);
-  p.rows = pairs * N;
-  if (p.use && p.splits > 1) {
-    p.ml_bytes = (p.rows * p.splits * 2 * (int64_t)sizeof(float) + 15) / 16 * 16;
-    p.bytes = p.ml_bytes + p.rows * p.splits * padded_dim(d.D) * (int64_t)sizeof(float);
+ForwardPlan forward_plan(const trace_attention_desc& d) {
+  ForwardPlan p{};
+  p.few = d.Lq <= 16;
+  if (p.few) {
+    const int64_t waves = ((int64_t)d.Lq * (d.Hq / d.Hk) + 31) / 32 * d.B * d.Hk;
+    const int64_t n = waves > 0 ? (1024 + waves - 1) / waves : 1, most = (d.Lk + 63) / 64;
+    p.splits = (int)(n < most ? n : most);
+    p.splits = p.splits < 1 ? 1 : p.splits < ATTN_MAX_SPLITS ? p.splits : ATTN_MAX_SPLITS;
+  } else {
+    p.splits = shares(items_of(d.Lq, (int64_t)d.B * d.Hq), (d.Lk + 63) / 64 / 2, 512);
+  }
+  if (p.splits > 1) {
+    const int64_t partial = (int64_t)d.B * d.Hq * d.Lq * p.splits;
+    p.ml_bytes = (partial * 2 * (int64_t)sizeof(float) + 15) / 16 * 16;
+    p.bytes = p.ml_bytes + partial * padded_dim(d.D) * (int64_t)sizeof(float);
   }
   return p;
 }
 
-// Shares of the dk / dv kernel's queries: enough for four workgroups a CU, each with at least 16 query tiles.
+// The backward pass: one kernel for short sequences, else the shares of its two kernels: four workgroups a CU, of at least two key
+// tiles (dq) or four query tiles (dk / dv) each.
 struct BackPlan {
-  bool whole;                        // short sequences: one kernel, no workspace
-  int splits;
-  int64_t delta_bytes, bytes;
+  bool whole;                        // short sequences: no workspace
+  int splits_q, splits;
+  int64_t delta_bytes, q_bytes, bytes;
 };
 BackPlan back_plan(const trace_attention_desc& d) {
-  const int64_t items = (int64_t)((d.Lk + 127) / 128) * d.Hk * d.B;
-  const int64_t list = (int64_t)((d.Lq + 31) / 32) * (d.Hq / d.Hk);
-  int64_t n = items > 0 ? (1024 + items - 1) / items : 1;
-  n = n < list / 16 ? n : list / 16;
   BackPlan p{};
   p.whole = d.Lq >= 1 && d.Lk >= 1 && d.Lq <= 64 && d.Lk <= 64;
   if (p.whole) return p;
-  p.splits = (int)(n < 1 ? 1 : n < 16 ? n : 16);
-  p.delta_bytes = ((int64_t)d.B * d.Hq * d.Lq * (int64_t)sizeof(float) + 15) / 16 * 16;
-  p.bytes = p.delta_bytes + (p.splits > 1 ? (int64_t)p.splits * 2 * d.B * d.Hk * d.Lk * padded_dim(d.D) * (int64_t)sizeof(float) : 0);
+  const int64_t hq = (int64_t)d.B * d.Hq, hk = (int64_t)d.B * d.Hk, row = padded_dim(d.D) * (int64_t)sizeof(float);
+  p.splits_q = shares(items_of(d.Lq, hq), (d.Lk + 63) / 64 / 2, 1024);
+  p.splits = shares(items_of(d.Lk, hk), (int64_t)((d.Lq + 31) / 32) * (d.Hq / d.Hk) / 4, 1024);
+  p.delta_bytes = (hq * d.Lq * (int64_t)sizeof(float) + 15) / 16 * 16;
+  p.q_bytes = p.splits_q > 1 ? p.splits_q * hq * d.Lq * row : 0;
+  p.bytes = p.delta_bytes + p.q_bytes + (p.splits > 1 ? p.splits * 2 * hk * d.Lk * row : 0);
   return p;
 }
 
@@ -109,7 +122,7 @@ extern "C" int64_t trace_attention_workspace_bytes(const trace_attention_desc* d
   const int rc = check_desc(d, "trace_attention_workspace_bytes");
   if (rc != TRACE_OK) return rc;
   if (d->B == 0 || d->Lq == 0) return 0;
-  return backward ? back_plan(*d).bytes : few_plan(*d).bytes;
+  return backward ? back_plan(*d).bytes : forward_plan(*d).bytes;
 }
 
 extern "C" int trace_attention(const trace_attention_desc* d, const void* q, const void* k, const void* v, void* out,
@@ -118,7 +131,7 @@ extern "C" int trace_attention(const trace_attention_desc* d, const void* q, con
   if (rc != TRACE_OK) return rc;
   if (d->B == 0 || d->Lq == 0) return TRACE_OK;
   TRACE_REQUIRE(q && out && lse && (d->Lk == 0 || (k && v)), "trace_attention: null argument");
-  const FewPlan plan = few_plan(*d);
+  const ForwardPlan plan = forward_plan(*d);
   if (plan.bytes > 0 && (!workspace || workspace_bytes < plan.bytes)) {
     set_error("trace_attention: workspace too small (%lld bytes, need %lld)", (long long)workspace_bytes,
               (long long)plan.bytes);
@@ -133,14 +146,12 @@ extern "C" int trace_attention(const trace_attention_desc* d, const void* q, con
   a.out = out; a.vo = c.view(d->out, out);
   a.lse = lse;
   a.vec = c.vec;
-  if (plan.use) {
-    a.splits = plan.splits;
-    a.part_ml = static_cast<float*>(workspace);
-    a.part_o = reinterpret_cast<float*>(static_cast<char*>(workspace) + plan.ml_bytes);
-    a.items = (int64_t)d->B * d->Hk * (((int64_t)d->Lq * a.G + 31) / 32) * plan.splits;
-    return by_type(d->dtype, AttnPass::few, a, (hipStream_t)stream);
-  }
-  return by_type(d->dtype, AttnPass::forward, a, (hipStream_t)stream);
+  a.splits = plan.splits;
+  a.part_ml = static_cast<float*>(workspace);
+  a.part_o = reinterpret_cast<float*>(static_cast<char*>(workspace) + plan.ml_bytes);
+  a.waves_q = waves_for(d->Lq);
+  a.items = (int64_t)d->B * d->Hk * (((int64_t)d->Lq * a.G + 31) / 32) * plan.splits;        // of attn_few_kernel
+  return by_type(d->dtype, plan.few ? AttnPass::few : AttnPass::forward, a, (hipStream_t)stream);
 }
 
 extern "C" int trace_attention_backward(const trace_attention_desc* d, const void* dout, const void* q, const void* k,
@@ -171,8 +182,12 @@ extern "C" int trace_attention_backward(const trace_attention_desc* d, const voi
   a.lse_in = lse;
   const BackPlan plan = back_plan(*d);
   a.delta = static_cast<float*>(workspace);
+  a.waves_q = waves_for(d->Lq);
+  a.waves_k = waves_for(d->Lk);
+  a.splits_q = plan.splits_q;
   a.splits = plan.splits;
-  a.part_o = reinterpret_cast<float*>(static_cast<char*>(workspace) + plan.delta_bytes);
+  a.part_q = reinterpret_cast<float*>(static_cast<char*>(workspace) + plan.delta_bytes);
+  a.part_o = reinterpret_cast<float*>(static_cast<char*>(workspace) + plan.delta_bytes + plan.q_bytes);
   a.vec = c.vec;
   if (plan.whole) return by_type(d->dtype, AttnPass::short_backward, a, (hipStream_t)stream);
   if (d->Lq > 0) {

@@ -34,7 +34,10 @@ struct AttnArgs {
   const unsigned char* key_mask;     // (B, Lk) or null
   long mask_stride;
   int vec;                           // every pointer and stride 16-byte aligned, D % 8 == 0
-  int splits;                        // ranges of keys (attn_few_kernel), shares of the queries (attn_dkv_kernel)
+  int waves_q, waves_k;              // waves of a workgroup over queries (forward, dq), over keys (dk / dv)
+  int splits_q;                      // shares of the keys (attn_dq_kernel), results in part_q: (splits_q, rows, padded D)
+  float* part_q;
+  int splits;                        // ranges of keys (forward), shares of the queries (attn_dkv_kernel)
   float *part_ml, *part_o;           // their partial results: (rows, splits, 2), (rows, splits, padded D) or
                                      // (splits, {dk, dv}, rows, padded D)
   long items;                        // work items of the launch
@@ -177,8 +180,26 @@ __device__ __forceinline__ long causal_start(const AttnArgs& a, int b) {
 template <typename T>
 constexpr int KEY_TILE = sizeof(T) == 4 ? 32 : 64;
 
+// Leaves one range's result of a row for attn_join_kernel: maximum and sum, and the unnormalised output (not written where
+// nothing was seen).  Rows are ordered (batch, key head, query, head of the group).
+template <typename T, int DP>
+__device__ __forceinline__ void put_partial(const AttnArgs& a, long row, int split, float m, float l, const f32x16 (&o)[DP / 32]) {
+  const int half = (threadIdx.x & 63) >> 5;
+  row = row * a.splits + split;
+  if (half == 0) reinterpret_cast<f32v2*>(a.part_ml)[row] = f32v2{m, l};
+  if (l == 0.f) return;
+  float* p = a.part_o + row * DP;
+#pragma unroll
+  for (int dt = 0; dt < DP / 32; ++dt)
+#pragma unroll
+    for (int g = 0; g < 4; ++g)
+      *reinterpret_cast<f32v4*>(p + dt * 32 + g * 8 + half * 4) =
+          f32v4{o[dt][4 * g], o[dt][4 * g + 1], o[dt][4 * g + 2], o[dt][4 * g + 3]};
+}
+
 // ---- forward ------------------------------------------------------------------------------------------------------
 // One workgroup = 32 NW queries of one head, one wave = 32 of them; the keys pass in tiles.
+// With few workgroups the tiles are cut into `splits` ranges, which attn_join_kernel joins.
 template <typename T, int DP, int NW>
 __global__ __launch_bounds__(NW * 64, sizeof(T) == 2 ? 2 : DP <= 64 ? 3 : 1) void attn_fwd_kernel(AttnArgs a) {
   typedef typename Elem<T>::V8 V8;
@@ -192,9 +213,10 @@ __global__ __launch_bounds__(NW * 64, sizeof(T) == 2 ? 2 : DP <= 64 ? 3 : 1) voi
   if (item >= a.items) return;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, col = lane & 31, half = lane >> 5;
   const int tiles = (a.Lq + 32 * NW - 1) / (32 * NW);
-  const int tile = tiles - 1 - (int)(item % tiles);       // causal: the longest first
-  const int hq = (int)((item / tiles) % a.Hq);
-  const int b = (int)(item / tiles / a.Hq);
+  const int split = (int)(item % a.splits);
+  const int tile = tiles - 1 - (int)(item / a.splits % tiles);       // causal: the longest first
+  const int hq = (int)((item / a.splits / tiles) % a.Hq);
+  const int b = (int)(item / a.splits / tiles / a.Hq);
   const int hk = hq / a.G;
   const int i = tile * 32 * NW + wave * 32 + col;         // this lane's query
   const bool vec = a.vec != 0;
@@ -214,6 +236,9 @@ __global__ __launch_bounds__(NW * 64, sizeof(T) == 2 ? 2 : DP <= 64 ? 3 : 1) voi
   const long seen = last_row + start + 1;                 // keys the last query of the workgroup sees
   const int end = (int)max(0L, min((long)len, seen));
   const long sees = (long)i + start;                      // last key this lane's query sees
+  const long all_tiles = (end + KT - 1) / KT;             // this workgroup's share of the key tiles
+  const int from = (int)(all_tiles * split / a.splits) * KT;
+  const int stop = (int)min((long)end, all_tiles * (split + 1) / a.splits * KT);
 
   const T* kb = (const T*)a.k + b * a.vk.sb + hk * a.vk.sh;
   const T* vb = (const T*)a.v + b * a.vv.sb + hk * a.vv.sh;
@@ -243,10 +268,10 @@ __global__ __launch_bounds__(NW * 64, sizeof(T) == 2 ? 2 : DP <= 64 ? 3 : 1) voi
 
   f32x16 o[ND] = {};
   float m = -INFINITY, l = 0.f;                            // l: the sum over this lane half's keys
-  unsigned long long bits = key_bits(a, b, 0, end) & FULL;
-  for (int key0 = 0; key0 < end; key0 += KT) {
+  unsigned long long bits = key_bits(a, b, from, end) & FULL;
+  for (int key0 = from; key0 < stop; key0 += KT) {
     const unsigned long long here = bits;
-    if (key0 + KT < end) bits = key_bits(a, b, key0 + KT, end) & FULL;
+    if (key0 + KT < stop) bits = key_bits(a, b, key0 + KT, end) & FULL;
     if (here == 0ull) continue;                            // the same in every wave
     __syncthreads();
     stage(key0, here);
@@ -309,6 +334,10 @@ __global__ __launch_bounds__(NW * 64, sizeof(T) == 2 ? 2 : DP <= 64 ? 3 : 1) voi
   }
   l += __shfl_xor(l, 32, 64);
   if (i >= a.Lq) return;
+  if (a.splits > 1) {
+    put_partial<T, DP>(a, (((long)b * a.Hk + hk) * a.Lq + i) * a.G + hq % a.G, split, m, l, o);
+    return;
+  }
   const float inv = l == 0.f ? 0.f : 1.f / l;
   T* op = (T*)a.out + b * a.vo.sb + hq * a.vo.sh + (long)i * a.vo.sl;
 #pragma unroll
@@ -450,17 +479,7 @@ __global__ __launch_bounds__(64) void attn_few_kernel(AttnArgs a) {
     if (half == 0) a.lse[((long)b * a.Hq + hq) * a.Lq + i] = l == 0.f ? -INFINITY : (m + log2f(l)) * LN2;
     return;
   }
-  // partial results: maximum and sum of the row's range, and its unnormalised output (not written where nothing was seen)
-  const long row = ((pair * N + n) * a.splits + split);
-  if (half == 0) reinterpret_cast<f32v2*>(a.part_ml)[row] = f32v2{m, l};
-  if (l == 0.f) return;
-  float* op = a.part_o + row * DP;
-#pragma unroll
-  for (int dt = 0; dt < ND; ++dt)
-#pragma unroll
-    for (int g = 0; g < 4; ++g)
-      *reinterpret_cast<f32v4*>(op + dt * 32 + g * 8 + half * 4) =
-          f32v4{o[dt][4 * g], o[dt][4 * g + 1], o[dt][4 * g + 2], o[dt][4 * g + 3]};
+  put_partial<T, DP>(a, pair * N + n, split, m, l, o);
 }
 
 // One workgroup joins the `splits` partial results of one query: out = sum_s 2^(m_s - M) o_s / sum_s 2^(m_s - M) l_s.
@@ -507,11 +526,48 @@ __global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a) {
   if (d == 0) a.lse[((long)b * a.Hq + hq) * a.Lq + i] = l == 0.f ? -INFINITY : (top + log2f(l)) * LN2;
 }
 
+// The same for up to ATTN_ROW_SPLITS ranges of many rows: a lane has four head elements of one row and every range of it
+// (16384 rows of 64 in 4 ranges: a quarter of the time of a workgroup a row).
+constexpr int ATTN_ROW_SPLITS = 16;
+template <typename T, int DP>
+__global__ __launch_bounds__(256) void attn_join_rows_kernel(AttnArgs a) {
+  constexpr int PER = DP / 4;
+  const long rows = (long)a.B * a.Hq * a.Lq;
+  const long at = (long)blockIdx.x * 256 + threadIdx.x, row = at / PER;
+  const int d = (int)(at % PER) * 4;
+  if (row >= rows || d >= a.D) return;
+  const f32v2* ml = reinterpret_cast<const f32v2*>(a.part_ml) + row * a.splits;
+  float top = -INFINITY;
+  for (int s = 0; s < a.splits; ++s) top = fmaxf(top, ml[s][0]);
+  const float use = top == -INFINITY ? 0.f : top;
+  float l = 0.f;
+  f32v4 t = {};
+#pragma unroll 4
+  for (int s = 0; s < a.splits; ++s) {
+    const f32v2 v = ml[s];
+    const f32v4 x = *reinterpret_cast<const f32v4*>(a.part_o + (row * a.splits + s) * DP + d);
+    const bool on = v[1] != 0.f;                           // else: nothing was written there
+    const float w = __builtin_amdgcn_exp2f(v[0] - use);
+    l += on ? w * v[1] : 0.f;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) t[e] += on ? w * x[e] : 0.f;
+  }
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) t[e] *= inv;
+  const long pair = row / ((long)a.Lq * a.G);
+  const int n = (int)(row % ((long)a.Lq * a.G)), i = n / a.G;
+  const int hk = (int)(pair % a.Hk), b = (int)(pair / a.Hk), hq = hk * a.G + n % a.G;
+  store4<T>((T*)a.out + b * a.vo.sb + hq * a.vo.sh + (long)i * a.vo.sl + d, t, a.D - d, a.vec);
+  if (d == 0) a.lse[((long)b * a.Hq + hq) * a.Lq + i] = l == 0.f ? -INFINITY : (top + log2f(l)) * LN2;
+}
+
 // ---- backward: dq (and delta) ---------------------------------------------------------------------------------------
 // One workgroup = 32 NW queries of one head, keys in tiles of KT: S^T and dP^T = V dO^T share the layout of the forward,
-// dq^T += K^T dS^T.  delta = dout . out is formed here first and left for the dk / dv kernel.
+// dq^T += K^T dS^T.  delta = dout . out is formed here first and left for the dk / dv kernel.  With few workgroups the key tiles
+// are cut into `splits_q` shares, whose fp32 results attn_sum_q_kernel adds in order.
 template <typename T, int DP, int NW>
-__global__ __launch_bounds__(NW * 64, sizeof(T) == 2 ? 2 : DP <= 64 ? 3 : 1) void attn_dq_kernel(AttnArgs a) {
+__global__ __launch_bounds__(NW * 64, sizeof(T) == 2 ? 2 : DP <= 32 ? 3 : DP <= 64 ? 2 : 1) void attn_dq_kernel(AttnArgs a) {
   typedef typename Elem<T>::V8 V8;
   constexpr int KT = KEY_TILE<T>, NT = NW * 64, NC = DP / 16, ND = DP / 32;
   constexpr int UN = KT / 4 * (DP / 8), UPT = (2 * UN + NT - 1) / NT;
@@ -524,9 +580,10 @@ __global__ __launch_bounds__(NW * 64, sizeof(T) == 2 ? 2 : DP <= 64 ? 3 : 1) voi
   if (item >= a.items) return;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, col = lane & 31, half = lane >> 5;
   const int tiles = (a.Lq + 32 * NW - 1) / (32 * NW);
-  const int tile = tiles - 1 - (int)(item % tiles);
-  const int hq = (int)((item / tiles) % a.Hq);
-  const int b = (int)(item / tiles / a.Hq);
+  const int split = (int)(item % a.splits_q);
+  const int tile = tiles - 1 - (int)(item / a.splits_q % tiles);
+  const int hq = (int)((item / a.splits_q / tiles) % a.Hq);
+  const int b = (int)(item / a.splits_q / tiles / a.Hq);
   const int hk = hq / a.G;
   const int i = tile * 32 * NW + wave * 32 + col;
   const bool vec = a.vec != 0;
@@ -547,13 +604,16 @@ __global__ __launch_bounds__(NW * 64, sizeof(T) == 2 ? 2 : DP <= 64 ? 3 : 1) voi
     for (int j = 0; j < 8; ++j) delta = fmaf((float)gf[c][j], (float)of[j], delta);
   }
   delta += __shfl_xor(delta, 32, 64);
-  if (half == 0 && i < a.Lq) a.delta[row] = delta;
+  if (half == 0 && i < a.Lq && split == 0) a.delta[row] = delta;
 
   const int len = key_limit(a, b);
   const long start = causal_start(a, b);
   const int last_row = min(tile * 32 * NW + 32 * NW, a.Lq) - 1;
   const int end = (int)max(0L, min((long)len, last_row + start + 1));
   const long sees = (long)i + start;
+  const long all_tiles = (end + KT - 1) / KT;             // this workgroup's share of the key tiles
+  const int from = (int)(all_tiles * split / a.splits_q) * KT;
+  const int stop = (int)min((long)end, all_tiles * (split + 1) / a.splits_q * KT);
   const T* kb = (const T*)a.k + b * a.vk.sb + hk * a.vk.sh;
   const T* vb = (const T*)a.v + b * a.vv.sb + hk * a.vv.sh;
   const bool whole = vec && a.D == DP && 2 * UN % NT == 0;
@@ -584,10 +644,10 @@ __global__ __launch_bounds__(NW * 64, sizeof(T) == 2 ? 2 : DP <= 64 ? 3 : 1) voi
     }
   };
   f32x16 acc[ND] = {};
-  unsigned long long bits = key_bits(a, b, 0, end) & FULL;
-  for (int key0 = 0; key0 < end; key0 += KT) {
+  unsigned long long bits = key_bits(a, b, from, end) & FULL;
+  for (int key0 = from; key0 < stop; key0 += KT) {
     const unsigned long long here = bits;
-    if (key0 + KT < end) bits = key_bits(a, b, key0 + KT, end) & FULL;
+    if (key0 + KT < stop) bits = key_bits(a, b, key0 + KT, end) & FULL;
     if (here == 0ull) continue;                            // the same in every wave
     __syncthreads();
     stage(key0, here);
@@ -623,6 +683,16 @@ __global__ __launch_bounds__(NW * 64, sizeof(T) == 2 ? 2 : DP <= 64 ? 3 : 1) voi
     }
   }
   if (i >= a.Lq) return;
+  if (a.splits_q > 1) {
+    float* p = a.part_q + (split * ((long)a.B * a.Hq * a.Lq) + row) * DP;
+#pragma unroll
+    for (int dt = 0; dt < ND; ++dt)
+#pragma unroll
+      for (int g = 0; g < 4; ++g)
+        *reinterpret_cast<f32v4*>(p + dt * 32 + g * 8 + half * 4) =
+            f32v4{acc[dt][4 * g], acc[dt][4 * g + 1], acc[dt][4 * g + 2], acc[dt][4 * g + 3]};
+    return;
+  }
   const float back = a.scale * P_UNSHIFT<T>;
   T* p = (T*)a.dq + b * a.vdq.sb + hq * a.vdq.sh + (long)i * a.vdq.sl;
 #pragma unroll
@@ -634,6 +704,27 @@ __global__ __launch_bounds__(NW * 64, sizeof(T) == 2 ? 2 : DP <= 64 ? 3 : 1) voi
                        acc[dt][4 * g + 3] * back};
       if (d < a.D) store4<T>(p + d, w, a.D - d, vec);
     }
+}
+
+// dq from the fp32 shares of the dq kernel; a lane has four head elements of one query.
+template <typename T, int DP>
+__global__ __launch_bounds__(256) void attn_sum_q_kernel(AttnArgs a) {
+  constexpr int PER = DP / 4;
+  const long rows = (long)a.B * a.Hq * a.Lq;
+  const long at = (long)blockIdx.x * 256 + threadIdx.x, row = at / PER;
+  const int d = (int)(at % PER) * 4;
+  if (row >= rows || d >= a.D) return;
+  f32v4 t = {};
+#pragma unroll 4
+  for (int s = 0; s < a.splits_q; ++s) {
+    const f32v4 x = *reinterpret_cast<const f32v4*>(a.part_q + (s * rows + row) * DP + d);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) t[e] += x[e];
+  }
+#pragma unroll
+  for (int e = 0; e < 4; ++e) t[e] *= a.scale * P_UNSHIFT<T>;
+  const int i = (int)(row % a.Lq), hq = (int)(row / a.Lq % a.Hq), b = (int)(row / a.Lq / a.Hq);
+  store4<T>((T*)a.dq + b * a.vdq.sb + hq * a.vdq.sh + (long)i * a.vdq.sl + d, t, a.D - d, a.vec);
 }
 
 // ---- backward: dk, dv ------------------------------------------------------------------------------------------------
@@ -670,8 +761,8 @@ __global__ __launch_bounds__(NW * 64, sizeof(T) == 2 || DP <= 64 ? 2 : 1) void a
   const int key0 = tile * 32 * NW;
   const int j = key0 + wave * 32 + col;                   // this lane's key
   const bool vec = a.vec != 0;
-  const int len = key_limit(a, b);
   const long start = causal_start(a, b);
+  const int len = (int)max(0L, min((long)key_limit(a, b), a.Lq + start));       // keys that no query sees count as absent
   const bool on = j < len && (!a.key_mask || a.key_mask[(long)b * a.mask_stride + j] != 0);
   V8 kf[NC], vf[V_LDS ? 1 : NC];
 #pragma unroll
@@ -883,8 +974,8 @@ __global__ __launch_bounds__(QB * KB * 64, DP == 32 || (DP == 64 && QB * KB == 4
   const int hk = (int)(item % a.Hk), b = (int)(item / a.Hk);
   const int qi = wave % QB, ki = wave / QB;
   const bool vec = a.vec != 0, whole_d = vec && a.D == DP;
-  const int len = key_limit(a, b);
   const long start = causal_start(a, b);
+  const int len = (int)max(0L, min((long)key_limit(a, b), a.Lq + start));       // keys behind count as absent
   const unsigned long long bits = key_bits(a, b, 0, len);
   const int i = qi * 32 + col;                                           // this lane's query
   const T* kb = (const T*)a.k + b * a.vk.sb + hk * a.vk.sh;

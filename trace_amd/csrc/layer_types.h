@@ -74,6 +74,7 @@ __device__ __forceinline__ void store4(T* p, f32v4 v, int n, bool vec) {
 
 // Workgroups are handed to the eight XCDs in turn; item() gives each XCD a contiguous range of the n work items, so that
 // items that read the same data meet in one L2.  Launch xcd_grid(n) workgroups; item() >= n: nothing to do.
+constexpr long MAX_GRID_THREADS = 0xffffffffL;              // of one launch
 constexpr long XCDS = 8;
 inline long xcd_grid(long n) { return (n + XCDS - 1) / XCDS * XCDS; }
 __device__ __forceinline__ long xcd_item(long n) {

@@ -14,6 +14,7 @@ struct NormArgs {
   const float *gate, *post, *weight, *bias;
   long xs, ys, dhs, dzs;             // row strides of the inputs; outputs are contiguous
   int R, C, rpc;                     // rows, columns, rows of a conditioning group
+  long row0;                         // forward: first row of the launch
   int layer;                         // 1: layer norm, 0: rms
   int cond, gate_cond;               // weight and bias / gate: one row per conditioning group (1) or one for all (0)
   float alpha, eps;
@@ -101,7 +102,7 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void residual_norm_kernel(No
   constexpr int NT = TPR < 256 ? 256 : TPR;
   __shared__ float red[2 * (NT / 64)];
   const int lane = threadIdx.x % TPR;
-  const long row = (long)blockIdx.x * (NT / TPR) + team_of<TPR>();
+  const long row = a.row0 + (long)blockIdx.x * (NT / TPR) + team_of<TPR>();
   if (row >= a.R) return;                                     // TPR > 64: a workgroup is one team
   int turn = 0;
   const int g = (int)(row / a.rpc);

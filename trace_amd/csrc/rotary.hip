@@ -164,7 +164,7 @@ extern "C" int trace_rotary(const trace_rotary_desc* d, const void* q, const voi
   // a sine for each lane, or one token
   a.per_wg = a.half >= 256 ? 1 : 256 / a.half;
   const long grid = (a.tokens + a.per_wg - 1) / a.per_wg;
-  TRACE_REQUIRE(grid < 0x7fffffffL, "trace_rotary: grid of %ld workgroups", grid);
+  TRACE_REQUIRE(grid * 256 <= MAX_GRID_THREADS, "trace_rotary: grid of %ld workgroups", grid);
   const size_t lds = (size_t)a.per_wg * a.half * sizeof(float2);
   const bool inter = d->interleaved != 0;
   hipStream_t st = (hipStream_t)stream;

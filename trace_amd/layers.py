@@ -226,6 +226,11 @@ def rotary(q, positions, freqs, k=None, interleaved=False, scale=1.0, inverse=Fa
         for name, t in (("q", q), ("k", k)):
             if t is not None and any(s == 0 and n > 1 for s, n in zip(t.stride(), t.shape)):
                 _refuse("%s is broadcast: it cannot be rotated in place", name)
+        if k is not None and q.stride() == k.stride():
+            # windows of one layout: apart by their heads, or side by side within a head's stride
+            head, apart = q.stride(2), (k.data_ptr() - q.data_ptr()) // q.element_size()
+            if -k.shape[2] * head < apart < Hq * head and not D <= apart % head <= head - D and q.numel() and k.numel():
+                _refuse("q and k share memory: they cannot be rotated in place together")
     _gpu(q)
     oq = q if inplace else torch.empty(q.shape, dtype=q.dtype, device=q.device)
     ok = k if k is None or inplace else torch.empty(k.shape, dtype=k.dtype, device=k.device)
