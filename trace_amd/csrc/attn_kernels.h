@@ -198,7 +198,10 @@ __device__ __forceinline__ void put_partial(const AttnArgs& a, long row, int spl
 }
 
 // ---- forward ------------------------------------------------------------------------------------------------------
-// One workgroup = 32 NW queries of one head, one wave = 32 of them; the keys pass in tiles.
+// One workgroup = 32 NW queries of one head, one wave = 32 of them; the keys pass in tiles.  8192 tokens, 16 on 4 heads of 128,
+// bf16, causal: 338 us, 813 TFLOP/s, the matrix pipe busy 37 %; a wave reads 32 KB of LDS for each 32 x 64 scores, which
+// takes as long as their products, so what is left is in more queries a wave.  Two waves a SIMD (603 us at one) and loads
+// between the barriers, not a tile ahead in registers (the same time, a fifth of the registers).
 // With few workgroups the tiles are cut into `splits` ranges, which attn_join_kernel joins.
 template <typename T, int DP, int NW>
 __global__ __launch_bounds__(NW * 64, sizeof(T) == 2 ? 2 : DP <= 64 ? 3 : 1) void attn_fwd_kernel(AttnArgs a) {
@@ -356,6 +359,7 @@ __global__ __launch_bounds__(NW * 64, sizeof(T) == 2 ? 2 : DP <= 64 ? 3 : 1) voi
 // with 32 columns and one of `splits` ranges of the sequence's keys, so a cache is read once and by the whole chip however
 // few its queries are; attn_join_kernel joins the ranges.  HBM-bound: per 32 keys a wave has 32 D elements of k (straight to the
 // operand's registers) and of v (transposed through LDS of its own, no barriers) in flight while it works on the last 32.
+// 8 sequences of up to 8192 keys, 32 on 8 heads of 128, bf16: 38 us, 5.3 TB/s (532 us in tiles of 32 queries a head).
 template <typename T, int DP>
 __global__ __launch_bounds__(64) void attn_few_kernel(AttnArgs a) {
   typedef typename Elem<T>::V8 V8;
@@ -565,7 +569,8 @@ __global__ __launch_bounds__(256) void attn_join_rows_kernel(AttnArgs a) {
 // ---- backward: dq (and delta) ---------------------------------------------------------------------------------------
 // One workgroup = 32 NW queries of one head, keys in tiles of KT: S^T and dP^T = V dO^T share the layout of the forward,
 // dq^T += K^T dS^T.  delta = dout . out is formed here first and left for the dk / dv kernel.  With few workgroups the key tiles
-// are cut into `splits_q` shares, whose fp32 results attn_sum_q_kernel adds in order.
+// are cut into `splits_q` shares, whose fp32 results attn_sum_q_kernel adds in order.  2 x 4001 tokens, 16 on 4 heads of 128,
+// bf16, causal: 345 us, 570 TFLOP/s of its three products (437 us with the next tile in registers, which spilled).
 template <typename T, int DP, int NW>
 __global__ __launch_bounds__(NW * 64, sizeof(T) == 2 ? 2 : DP <= 32 ? 3 : DP <= 64 ? 2 : 1) void attn_dq_kernel(AttnArgs a) {
   typedef typename Elem<T>::V8 V8;
@@ -735,7 +740,8 @@ constexpr bool DKV_V_LDS = sizeof(T) == 2 && DP == 128;
 
 // One workgroup = 32 NW keys of one key head, one wave = 32 of them; the queries of every head that shares it pass in
 // tiles of 32.  S and dP = dO V^T here have queries as rows: dv^T += dO^T P, dk^T += Q^T dS.  The sums over heads
-// and queries stay in one accumulator in a fixed order: no atomics, the same bits every time.
+// and queries stay in one accumulator in a fixed order: no atomics, the same bits every time.  2 x 4001 tokens, 16 on 4 heads
+// of 128, bf16, causal: 460 us, 570 TFLOP/s of its four products (1440 us without shares and at one wave a SIMD).
 template <typename T, int DP, int NW>
 __global__ __launch_bounds__(NW * 64, sizeof(T) == 2 || DP <= 64 ? 2 : 1) void attn_dkv_kernel(AttnArgs a) {
   typedef typename Elem<T>::V8 V8;
@@ -917,7 +923,8 @@ __global__ __launch_bounds__(NW * 64, sizeof(T) == 2 || DP <= 64 ? 2 : 1) void a
 // are formed once (5 products instead of 7).  Wave (qi, ki) forms the 32x32 block of S^T and dP^T of its queries and keys;
 // P, then dS, pass through LDS to the waves that own the 32x32 tiles of dv^T, dk^T and dq^T.  All tiles are token-major
 // (TileN): an operand that runs along the tokens is read element by element, lanes side by side.  dk and dv stay in registers
-// over the query heads of the group.
+// over the query heads of the group.  fp32, L = 52, D = 64: loads and stores alone take 1024 us of the 1680, the matrix
+// instructions 745; the two workgroups that a CU's LDS holds do not overlap them.
 template <typename T, int W>
 struct TileN {
   static constexpr int S = W + 8;      // rows 4 apart start half the banks apart, rows 1 apart 16 or 32 bytes
@@ -938,27 +945,21 @@ __device__ __forceinline__ typename Elem<T>::V8 frag_rows(const T* p, int stride
   return v;
 }
 
-// acc += sum over c < N of mma32(A(c), B(c)), the operands of step c + 1 read from LDS while step c runs: left to itself the
-// compiler waits for every read right before its use, which idles the matrix pipe for half of an LDS latency each time.
+// acc += sum over c < N of mma32(A(c), B(c)).
 template <typename T, int N, typename FA, typename FB>
-__device__ __forceinline__ void mma_ahead(f32x16& acc, FA fa, FB fb) {
-  typename Elem<T>::V8 x[2], y[2];
-  x[0] = fa(0);
-  y[0] = fb(0);
+__device__ __forceinline__ void mma_sum(f32x16& acc, FA fa, FB fb) {
 #pragma unroll
-  for (int c = 0; c < N; ++c) {
-    if (c + 1 < N) {
-      x[(c + 1) & 1] = fa(c + 1);
-      y[(c + 1) & 1] = fb(c + 1);
-    }
-    __builtin_amdgcn_sched_barrier(0);
-    acc = Elem<T>::mma32(x[c & 1], y[c & 1], acc);
-    __builtin_amdgcn_sched_barrier(0);
-  }
+  for (int c = 0; c < N; ++c) acc = Elem<T>::mma32(fa(c), fb(c), acc);
 }
 
+// Waves a SIMD that the registers are cut to: what measured best (10240 sequences of 52 steps, 4 heads of 64: bf16 732 us, fp32 1680;
+// of 24 steps, bf16: 342 us at two waves, 391 at one).  Three waves of fp32, four of 32-element heads spill and are half as fast.
 template <typename T, int DP, int QB, int KB>
-__global__ __launch_bounds__(QB * KB * 64, DP == 32 || (DP == 64 && QB * KB == 4) ? 2 : 1) void attn_short_backward_kernel(AttnArgs a) {
+constexpr int SHORT_WAVES = sizeof(T) == 2 ? (DP == 32 ? 3 : DP == 64 || QB * KB == 4 ? 2 : 1)
+                                           : (DP == 32 || (DP == 64 && QB * KB == 4) ? 2 : 1);
+
+template <typename T, int DP, int QB, int KB>
+__global__ __launch_bounds__(QB * KB * 64, (SHORT_WAVES<T, DP, QB, KB>)) void attn_short_backward_kernel(AttnArgs a) {
   typedef typename Elem<T>::V8 V8;
   constexpr int NW = QB * KB, NT = NW * 64, NC = DP / 16, ND = DP / 32, S = TileN<T, DP>::S, XS = TileN<T, 32 * KB>::S;
   constexpr int UQ = 8 * QB * (DP / 8), UK = 8 * KB * (DP / 8);          // staging units of a query / key tile
@@ -1053,9 +1054,9 @@ __global__ __launch_bounds__(QB * KB * 64, DP == 32 || (DP == 64 && QB * KB == 4
     __syncthreads();
     f32x16 s = {}, dp = {};
     float delta = 0.f;
-    mma_ahead<T, NC>(s, [&](int c) { return *reinterpret_cast<const V8*>(kt + (ki * 32 + col) * S + c * 16 + half * 8); },
+    mma_sum<T, NC>(s, [&](int c) { return *reinterpret_cast<const V8*>(kt + (ki * 32 + col) * S + c * 16 + half * 8); },
                      [&](int c) { return *reinterpret_cast<const V8*>(qt + i * S + c * 16 + half * 8); });
-    mma_ahead<T, NC>(dp, [&](int c) { return vf[c]; }, [&](int c) {
+    mma_sum<T, NC>(dp, [&](int c) { return vf[c]; }, [&](int c) {
       const V8 gf = *reinterpret_cast<const V8*>(gt + i * S + c * 16 + half * 8);
 #pragma unroll
       for (int j = 0; j < 8; ++j) delta = fmaf((float)gf[j], (float)of[c][j], delta);
@@ -1086,7 +1087,7 @@ __global__ __launch_bounds__(QB * KB * 64, DP == 32 || (DP == 64 && QB * KB == 4
     for (int n = 0; n < KTILES; ++n) {
       const int t = wave + n * NW;
       if (KB * ND % NW == 0 || t < KB * ND) {
-        mma_ahead<T, 2 * QB>(dv[n], [&](int c) { return frag_rows<T>(gt + c * 16 * S + t % ND * 32 + col, S, half); },
+        mma_sum<T, 2 * QB>(dv[n], [&](int c) { return frag_rows<T>(gt + c * 16 * S + t % ND * 32 + col, S, half); },
                              [&](int c) { return frag_rows<T>(xt + c * 16 * XS + t / ND * 32 + col, XS, half); });
       }
     }
@@ -1097,7 +1098,7 @@ __global__ __launch_bounds__(QB * KB * 64, DP == 32 || (DP == 64 && QB * KB == 4
     for (int n = 0; n < KTILES; ++n) {
       const int t = wave + n * NW;
       if (KB * ND % NW == 0 || t < KB * ND) {
-        mma_ahead<T, 2 * QB>(dk[n], [&](int c) { return frag_rows<T>(qt + c * 16 * S + t % ND * 32 + col, S, half); },
+        mma_sum<T, 2 * QB>(dk[n], [&](int c) { return frag_rows<T>(qt + c * 16 * S + t % ND * 32 + col, S, half); },
                              [&](int c) { return frag_rows<T>(xt + c * 16 * XS + t / ND * 32 + col, XS, half); });
       }
     }
@@ -1106,7 +1107,7 @@ __global__ __launch_bounds__(QB * KB * 64, DP == 32 || (DP == 64 && QB * KB == 4
       const int t = wave + n * NW;
       if (QB * ND % NW == 0 || t < QB * ND) {
         f32x16 dq = {};
-        mma_ahead<T, 2 * KB>(dq, [&](int c) { return frag_rows<T>(kt + c * 16 * S + t % ND * 32 + col, S, half); },
+        mma_sum<T, 2 * KB>(dq, [&](int c) { return frag_rows<T>(kt + c * 16 * S + t % ND * 32 + col, S, half); },
                              [&](int c) { return frag_slots<T>(xt + (t / ND * 32 + col) * XS + c * 16, half); });
         const int row = t / ND * 32 + col;
         T* p = (T*)a.dq + b * a.vdq.sb + hq * a.vdq.sh + (long)row * a.vdq.sl;
