@@ -123,14 +123,33 @@ __device__ __forceinline__ const typename Elem<T>::V8 frag_at(const T* tile, int
   return *reinterpret_cast<const typename Elem<T>::V8*>(tile + at);
 }
 
-// Registers 8c .. 8c + 7 of a 32x32 result as the second operand of the next product (16 of its 32 rows).  The only
-// rounding of P and dS: to the inputs' type, to nearest, as the matrix instruction takes no wider operand.
+// Registers 8c .. 8c + 7 of a 32x32 result as the second operand of the next product (16 of its 32 rows).  With T a 16-bit type,
+// the only rounding of P and dS: to the inputs' type, to nearest, as the matrix instruction takes no wider operand.  It adds as
+// much to the error of a result as its own rounding to the type does.
 template <typename T>
 __device__ __forceinline__ typename Elem<T>::V8 as_operand(const f32x16& s, int c) {
   typename Elem<T>::V8 v;
 #pragma unroll
   for (int i = 0; i < 8; ++i) v[i] = (T)s[8 * c + i];
   return v;
+}
+
+// c += a b with b in fp32: 16-bit types take b as the sum of two operands, each rounded to the type, and so lose nothing of it
+// that their results could show.  For kernels whose matrix instructions are not what bounds them.
+template <typename T>
+__device__ __forceinline__ f32x16 mma_wide(typename Elem<T>::V8 a, f32v8 b, f32x16 c) {
+  typename Elem<T>::V8 high, low;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    high[i] = (T)b[i];
+    low[i] = (T)(b[i] - (float)high[i]);
+  }
+  c = Elem<T>::mma32(a, high, c);
+  return Elem<T>::mma32(a, low, c);
+}
+template <>
+__device__ __forceinline__ f32x16 mma_wide<float>(f32v8 a, f32v8 b, f32x16 c) {
+  return Elem<float>::mma32(a, b, c);
 }
 
 // fp16: P and dS are rounded as 16 P and 16 dS.  A row of n keys holds P of about 1 / n, which from n = 2^14 on, and dS sooner,
@@ -201,7 +220,7 @@ __device__ __forceinline__ void put_partial(const AttnArgs& a, long row, int spl
 // One workgroup = 32 NW queries of one head, one wave = 32 of them; the keys pass in tiles.  8192 tokens, 16 on 4 heads of 128,
 // bf16, causal: 338 us, 813 TFLOP/s, the matrix pipe busy 37 %; a wave reads 32 KB of LDS for each 32 x 64 scores, which
 // takes as long as their products, so what is left is in more queries a wave.  Two waves a SIMD (603 us at one) and loads
-// between the barriers, not a tile ahead in registers (the same time, a fifth of the registers).
+// between the barriers, not a tile ahead in registers (which took a fifth more of them for the same time).
 // With few workgroups the tiles are cut into `splits` ranges, which attn_join_kernel joins.
 template <typename T, int DP, int NW>
 __global__ __launch_bounds__(NW * 64, sizeof(T) == 2 ? 2 : DP <= 64 ? 3 : 1) void attn_fwd_kernel(AttnArgs a) {
@@ -461,10 +480,10 @@ __global__ __launch_bounds__(64) void attn_few_kernel(AttnArgs a) {
     }
 #pragma unroll
     for (int c = 0; c < 2; ++c) {
-      const V8 p = as_operand<T>(s, c);
+      const f32v8 p = as_operand<float>(s, c);
 #pragma unroll
       for (int dt = 0; dt < ND; ++dt)
-        o[dt] = Elem<T>::mma32(frag_at<T>(vx, TileX<T, KT>::frag(dt * 32 + col, c, half)), p, o[dt]);
+        o[dt] = mma_wide<T>(frag_at<T>(vx, TileX<T, KT>::frag(dt * 32 + col, c, half)), p, o[dt]);
     }
   }
   l += __shfl_xor(l, 32, 64);
@@ -921,7 +940,7 @@ __global__ __launch_bounds__(NW * 64, sizeof(T) == 2 || DP <= 64 ? 2 : 1) void a
 // ---- backward of short sequences -------------------------------------------------------------------------------------
 // At most 32 QB queries and 32 KB keys: one workgroup does a whole key head, so that every tensor crosses HBM once and S, dP
 // are formed once (5 products instead of 7).  Wave (qi, ki) forms the 32x32 block of S^T and dP^T of its queries and keys;
-// P, then dS, pass through LDS to the waves that own the 32x32 tiles of dv^T, dk^T and dq^T.  All tiles are token-major
+// P, then dS, pass through LDS, in fp32, to the waves that own the 32x32 tiles of dv^T, dk^T and dq^T.  All tiles are token-major
 // (TileN): an operand that runs along the tokens is read element by element, lanes side by side.  dk and dv stay in registers
 // over the query heads of the group.  fp32, L = 52, D = 64: loads and stores alone take 1024 us of the 1680, the matrix
 // instructions 745; the two workgroups that a CU's LDS holds do not overlap them.
@@ -929,11 +948,9 @@ template <typename T, int W>
 struct TileN {
   static constexpr int S = W + 8;      // rows 4 apart start half the banks apart, rows 1 apart 16 or 32 bytes
 };
-// eight elements along a row, in slot order (token-major source, contraction along the row)
-template <typename T>
-__device__ __forceinline__ typename Elem<T>::V8 frag_slots(const T* p, int half) {
-  const typename Elem<T>::V4 u = *reinterpret_cast<const typename Elem<T>::V4*>(p + 4 * half);
-  const typename Elem<T>::V4 v = *reinterpret_cast<const typename Elem<T>::V4*>(p + 8 + 4 * half);
+// eight fp32 elements along a row, in slot order (contraction along the row)
+__device__ __forceinline__ f32v8 frag_slots(const float* p, int half) {
+  const f32v4 u = *reinterpret_cast<const f32v4*>(p + 4 * half), v = *reinterpret_cast<const f32v4*>(p + 8 + 4 * half);
   return __builtin_shufflevector(u, v, 0, 1, 2, 3, 4, 5, 6, 7);
 }
 // eight rows in slot order, one column (contraction along the tokens); p: row 0 of the group of 16, this lane's column
@@ -945,30 +962,22 @@ __device__ __forceinline__ typename Elem<T>::V8 frag_rows(const T* p, int stride
   return v;
 }
 
-// acc += sum over c < N of mma32(A(c), B(c)).
-template <typename T, int N, typename FA, typename FB>
-__device__ __forceinline__ void mma_sum(f32x16& acc, FA fa, FB fb) {
-#pragma unroll
-  for (int c = 0; c < N; ++c) acc = Elem<T>::mma32(fa(c), fb(c), acc);
-}
-
-// Waves a SIMD that the registers are cut to: what measured best (10240 sequences of 52 steps, 4 heads of 64: bf16 732 us, fp32 1680;
-// of 24 steps, bf16: 342 us at two waves, 391 at one).  Three waves of fp32, four of 32-element heads spill and are half as fast.
+// Waves a SIMD that the registers are cut to: what measured best (10240 sequences of 52 steps, 4 heads of 64: bf16 774 us, fp32 1680;
+// of 24 steps, bf16: 325 us at two waves, 391 at one).  Where more waves would spill they are slower, by half and more.
 template <typename T, int DP, int QB, int KB>
-constexpr int SHORT_WAVES = sizeof(T) == 2 ? (DP == 32 ? 3 : DP == 64 || QB * KB == 4 ? 2 : 1)
-                                           : (DP == 32 || (DP == 64 && QB * KB == 4) ? 2 : 1);
+constexpr int SHORT_WAVES = sizeof(T) == 2 ? (DP == 32 ? 3 : DP == 64 ? 2 : 1) : (DP == 32 || (DP == 64 && QB * KB == 4) ? 2 : 1);
 
 template <typename T, int DP, int QB, int KB>
 __global__ __launch_bounds__(QB * KB * 64, (SHORT_WAVES<T, DP, QB, KB>)) void attn_short_backward_kernel(AttnArgs a) {
   typedef typename Elem<T>::V8 V8;
-  constexpr int NW = QB * KB, NT = NW * 64, NC = DP / 16, ND = DP / 32, S = TileN<T, DP>::S, XS = TileN<T, 32 * KB>::S;
+  constexpr int NW = QB * KB, NT = NW * 64, NC = DP / 16, ND = DP / 32, S = TileN<T, DP>::S, XS = TileN<float, 32 * KB>::S;
   constexpr int UQ = 8 * QB * (DP / 8), UK = 8 * KB * (DP / 8);          // staging units of a query / key tile
   constexpr int KTILES = (KB * ND + NW - 1) / NW, QTILES = (QB * ND + NW - 1) / NW;
   extern __shared__ __attribute__((aligned(16))) char lds[];
   T* const qt = reinterpret_cast<T*>(lds);
   T* const gt = qt + 32 * QB * S;
   T* const kt = gt + 32 * QB * S;
-  T* const xt = kt + 32 * KB * S;                                        // P, then dS: (query, key)
+  float* const xt = reinterpret_cast<float*>(kt + 32 * KB * S);          // P, then dS: (query, key)
   const long item = xcd_item(a.items);
   if (item >= a.items) return;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, col = lane & 31, half = lane >> 5;
@@ -1054,14 +1063,15 @@ __global__ __launch_bounds__(QB * KB * 64, (SHORT_WAVES<T, DP, QB, KB>)) void at
     __syncthreads();
     f32x16 s = {}, dp = {};
     float delta = 0.f;
-    mma_sum<T, NC>(s, [&](int c) { return *reinterpret_cast<const V8*>(kt + (ki * 32 + col) * S + c * 16 + half * 8); },
-                     [&](int c) { return *reinterpret_cast<const V8*>(qt + i * S + c * 16 + half * 8); });
-    mma_sum<T, NC>(dp, [&](int c) { return vf[c]; }, [&](int c) {
-      const V8 gf = *reinterpret_cast<const V8*>(gt + i * S + c * 16 + half * 8);
+#pragma unroll
+    for (int c = 0; c < NC; ++c) {
+      const int at = c * 16 + half * 8;
+      s = Elem<T>::mma32(*reinterpret_cast<const V8*>(kt + (ki * 32 + col) * S + at), *reinterpret_cast<const V8*>(qt + i * S + at), s);
+      const V8 gf = *reinterpret_cast<const V8*>(gt + i * S + at);
+      dp = Elem<T>::mma32(vf[c], gf, dp);
 #pragma unroll
       for (int j = 0; j < 8; ++j) delta = fmaf((float)gf[j], (float)of[c][j], delta);
-      return gf;
-    });
+    }
     delta += __shfl_xor(delta, 32, 64);
     delta = live ? delta : 0.f;
     {
@@ -1078,7 +1088,7 @@ __global__ __launch_bounds__(QB * KB * 64, (SHORT_WAVES<T, DP, QB, KB>)) void at
     auto put = [&](const f32x16& x) {
 #pragma unroll
       for (int q = 0; q < 4; ++q)
-        store4<T>(xt + i * XS + ki * 32 + 8 * q + 4 * half, f32v4{x[4 * q], x[4 * q + 1], x[4 * q + 2], x[4 * q + 3]}, 4, true);
+        *reinterpret_cast<f32v4*>(xt + i * XS + ki * 32 + 8 * q + 4 * half) = f32v4{x[4 * q], x[4 * q + 1], x[4 * q + 2], x[4 * q + 3]};
     };
     // tile t of a gradient: token block t / ND, head elements 32 (t % ND) .. + 31
     put(s);
@@ -1087,8 +1097,10 @@ __global__ __launch_bounds__(QB * KB * 64, (SHORT_WAVES<T, DP, QB, KB>)) void at
     for (int n = 0; n < KTILES; ++n) {
       const int t = wave + n * NW;
       if (KB * ND % NW == 0 || t < KB * ND) {
-        mma_sum<T, 2 * QB>(dv[n], [&](int c) { return frag_rows<T>(gt + c * 16 * S + t % ND * 32 + col, S, half); },
-                             [&](int c) { return frag_rows<T>(xt + c * 16 * XS + t / ND * 32 + col, XS, half); });
+#pragma unroll
+        for (int c = 0; c < 2 * QB; ++c)
+          dv[n] = mma_wide<T>(frag_rows<T>(gt + c * 16 * S + t % ND * 32 + col, S, half),
+                              frag_rows<float>(xt + c * 16 * XS + t / ND * 32 + col, XS, half), dv[n]);
       }
     }
     __syncthreads();
@@ -1098,8 +1110,10 @@ __global__ __launch_bounds__(QB * KB * 64, (SHORT_WAVES<T, DP, QB, KB>)) void at
     for (int n = 0; n < KTILES; ++n) {
       const int t = wave + n * NW;
       if (KB * ND % NW == 0 || t < KB * ND) {
-        mma_sum<T, 2 * QB>(dk[n], [&](int c) { return frag_rows<T>(qt + c * 16 * S + t % ND * 32 + col, S, half); },
-                             [&](int c) { return frag_rows<T>(xt + c * 16 * XS + t / ND * 32 + col, XS, half); });
+#pragma unroll
+        for (int c = 0; c < 2 * QB; ++c)
+          dk[n] = mma_wide<T>(frag_rows<T>(qt + c * 16 * S + t % ND * 32 + col, S, half),
+                              frag_rows<float>(xt + c * 16 * XS + t / ND * 32 + col, XS, half), dk[n]);
       }
     }
 #pragma unroll
@@ -1107,8 +1121,10 @@ __global__ __launch_bounds__(QB * KB * 64, (SHORT_WAVES<T, DP, QB, KB>)) void at
       const int t = wave + n * NW;
       if (QB * ND % NW == 0 || t < QB * ND) {
         f32x16 dq = {};
-        mma_sum<T, 2 * KB>(dq, [&](int c) { return frag_rows<T>(kt + c * 16 * S + t % ND * 32 + col, S, half); },
-                             [&](int c) { return frag_slots<T>(xt + (t / ND * 32 + col) * XS + c * 16, half); });
+#pragma unroll
+        for (int c = 0; c < 2 * KB; ++c)
+          dq = mma_wide<T>(frag_rows<T>(kt + c * 16 * S + t % ND * 32 + col, S, half),
+                           frag_slots(xt + (t / ND * 32 + col) * XS + c * 16, half), dq);
         const int row = t / ND * 32 + col;
         T* p = (T*)a.dq + b * a.vdq.sb + hq * a.vdq.sh + (long)row * a.vdq.sl;
 #pragma unroll

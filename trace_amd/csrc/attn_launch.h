@@ -76,7 +76,7 @@ template <typename T, int DP, int QB, int KB>
 int short_backward(AttnArgs a, hipStream_t st) {
   static unsigned long long attr = 0;
   a.items = (long)a.Hk * a.B;
-  const size_t lds = sizeof(T) * ((2 * QB + KB) * 32 * TileN<T, DP>::S + 32 * QB * TileN<T, 32 * KB>::S);
+  const size_t lds = sizeof(T) * (2 * QB + KB) * 32 * TileN<T, DP>::S + sizeof(float) * 32 * QB * TileN<float, 32 * KB>::S;
   return launch(&attn_short_backward_kernel<T, DP, QB, KB>, &attr, lds, QB * KB * 64, a, st, "attn_short_backward_kernel");
 }
 template <typename T, int DP>
