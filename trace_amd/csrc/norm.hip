@@ -20,7 +20,7 @@ bool plan_for(int C, int es_x, int es_y, bool vec, NormPlan* p) {
   p->tpr = C <= 1024 ? 64 : C <= 4096 ? 256 : 1024;
   p->teams_wg = p->tpr == 64 ? 4 : 1;
   if (p->v == 1) {
-    p->k = 16;
+    p->k = p->tpr > 64 ? (C <= 8 * p->tpr ? 8 : 16) : C <= 64 ? 1 : C <= 256 ? 4 : 16;
   } else {
     p->k = 1;
     while (p->tpr * p->v * p->k < C) p->k *= 2;
@@ -43,7 +43,12 @@ int run(bool back, const NormArgs& a, int grid, hipStream_t st) {
 template <typename TX, typename TY, int TPR>
 int run_tpr(bool back, const NormPlan& p, const NormArgs& a, int grid, hipStream_t st) {
   constexpr int W = sizeof(TX) == 2 && sizeof(TY) == 2 ? 8 : 4, KM = 16 / W;
-  if (p.v == 1) return run<TX, TY, TPR, 1, 16>(back, a, grid, st);
+  if (p.v == 1) {
+    if (p.k == 16) return run<TX, TY, TPR, 1, 16>(back, a, grid, st);
+    if (TPR > 64) return run<TX, TY, TPR, 1, (TPR > 64 ? 8 : 16)>(back, a, grid, st);
+    return p.k == 4 ? run<TX, TY, TPR, 1, (TPR > 64 ? 16 : 4)>(back, a, grid, st)
+                    : run<TX, TY, TPR, 1, (TPR > 64 ? 16 : 1)>(back, a, grid, st);
+  }
   if (p.k == KM) return run<TX, TY, TPR, W, KM>(back, a, grid, st);
   if (p.k == KM / 2) return run<TX, TY, TPR, W, KM / 2>(back, a, grid, st);
   return run<TX, TY, TPR, W, 1>(back, a, grid, st);
@@ -109,7 +114,8 @@ BackPlan back_plan(const trace_norm_desc& d, int tpr, int teams_wg) {
   b.groups = (int)(((int64_t)d.rows + d.rows_per_cond - 1) / d.rows_per_cond);
   const int rpc = d.rows_per_cond < d.rows ? d.rows_per_cond : d.rows;
   int nsub = target / b.groups;
-  nsub = nsub < 1 ? 1 : nsub > rpc ? rpc : nsub;
+  const int most = (rpc + 1) / 2;                            // two rows at least: with few rows it is a team's rows one by one that take the time
+  nsub = nsub < 1 ? 1 : nsub > most ? most : nsub;
   b.rows_sub = (rpc + nsub - 1) / nsub;
   b.nsub = (rpc + b.rows_sub - 1) / b.rows_sub;
   b.chunks = b.groups * b.nsub;
@@ -122,10 +128,11 @@ BackPlan back_plan(const trace_norm_desc& d, int tpr, int teams_wg) {
   return b;
 }
 
-int reduce(const float* part, float* out, int groups, int n, int C, hipStream_t st) {
-  const long grid = (long)groups * ((C + 63) / 64);
+int reduce(const NormReduceArgs& a, hipStream_t st) {
+  if (a.count == 0) return TRACE_OK;
+  const long grid = (long)a.count * a.groups * ((a.C + 63) / 64);
   TRACE_REQUIRE(grid * 1024 <= MAX_GRID_THREADS, "norm_reduce_kernel: grid of %ld workgroups", grid);
-  hipLaunchKernelGGL(norm_reduce_kernel, dim3((unsigned)grid), dim3(1024), 0, st, part, out, n, C);
+  hipLaunchKernelGGL(norm_reduce_kernel, dim3((unsigned)grid), dim3(1024), 0, st, a);
   return launch_status("norm_reduce_kernel");
 }
 
@@ -205,14 +212,20 @@ extern "C" int trace_residual_norm_backward(const trace_norm_desc* d, const void
   a.part_g = a.part_s + 4 * b.part_s;
   a.nsub = b.nsub; a.rows_sub = b.rows_sub; a.chunks = b.chunks; a.per_team = b.per_team;
   int r = dispatch(true, *d, p, a, b.wgs, st);
-  float* const grads[3] = {dgate, dweight, dbias};
-  for (int i = 0; i < 3 && r == TRACE_OK; ++i) {
+  float* const grads[4] = {dgate, dweight, dbias, dpost_weight};
+  NormReduceArgs shared{}, cond{};
+  shared.groups = 1; shared.n = b.wgs; shared.C = d->C;
+  cond.groups = b.groups; cond.n = b.nsub; cond.C = d->C;
+  for (int i = 0; i < 4; ++i) {
     if (!grads[i]) continue;
-    if (!(i > 0 ? a.cond : a.gate_cond))
-      r = reduce(a.part_s + i * b.part_s, grads[i], 1, b.wgs, d->C, st);
-    else if (b.nsub > 1)
-      r = reduce(a.part_g + i * b.part_g, grads[i], b.groups, b.nsub, d->C, st);
+    if (i == 3 || !(i > 0 ? a.cond : a.gate_cond)) {
+      shared.part[shared.count] = a.part_s + i * b.part_s;
+      shared.out[shared.count++] = grads[i];
+    } else if (b.nsub > 1) {
+      cond.part[cond.count] = a.part_g + i * b.part_g;
+      cond.out[cond.count++] = grads[i];
+    }
   }
-  if (r == TRACE_OK && dpost_weight) r = reduce(a.part_s + 3 * b.part_s, dpost_weight, 1, b.wgs, d->C, st);
-  return r;
+  if (r == TRACE_OK) r = reduce(shared, st);
+  return r == TRACE_OK ? reduce(cond, st) : r;
 }

@@ -337,22 +337,32 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void residual_norm_backward_
   }
 }
 
-// out[g][c] = sum of rows g n .. g n + n - 1 of part, in a fixed order: 16 row lanes, then their sums in order.
-__global__ __launch_bounds__(1024) void norm_reduce_kernel(const float* part, float* out, int n, int C) {
+// out[i][g][c] = sum of rows g n .. g n + n - 1 of part[i], in a fixed order: 16 row lanes, then their sums in order.  All of a
+// call's sums of one kind in one launch.
+struct NormReduceArgs {
+  const float* part[4];
+  float* out[4];
+  int count, groups, n, C;
+};
+__global__ __launch_bounds__(1024) void norm_reduce_kernel(NormReduceArgs a) {
   __shared__ float s[16][64];
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-  const int blocks = (C + 63) / 64;
-  const long g = blockIdx.x / blocks;
+  const int blocks = (a.C + 63) / 64;
+  const int at = blockIdx.x / blocks, i = at / a.groups;
+  const long g = at % a.groups;
   const int c = (int)(blockIdx.x % blocks) * 64 + lane;
+  const float* p = a.part[i] + g * a.n * a.C + c;
   float t = 0.f;
-  if (c < C)
-    for (int r = w; r < n; r += 16) t += part[(g * n + r) * C + c];
+  if (c < a.C) {
+#pragma unroll 8
+    for (int r = w; r < a.n; r += 16) t += p[(long)r * a.C];
+  }
   s[w][lane] = t;
   __syncthreads();
-  if (w == 0 && c < C) {
+  if (w == 0 && c < a.C) {
 #pragma unroll
     for (int k = 1; k < 16; ++k) t += s[k][lane];
-    out[g * C + c] = t;
+    a.out[i][g * a.C + c] = t;
   }
 }
 
