@@ -13,7 +13,8 @@ struct NormPlan {
 };
 
 // The narrowest team that holds a row in 16 elements a lane: a wave up to 1024 columns (no barrier in its sums), 256 lanes
-// up to 4096, 1024 lanes up to 16384.  Vectors are 16 bytes of the narrower type where C and all addresses allow.
+// up to 4096, 1024 lanes up to 16384.  Vectors are 16 bytes where C and all addresses allow (8 of a 16-bit type beside an fp32
+// stream), single elements else, as many as the row needs (20448 x 1637 fp32, backward: 501 us, 946 with 16 for every row).
 bool plan_for(int C, int es_x, int es_y, bool vec, NormPlan* p) {
   const int wide = es_x == 2 && es_y == 2 ? 8 : 4;
   p->v = vec && C % wide == 0 ? wide : 1;
