@@ -77,8 +77,8 @@ template <typename T>
 struct Unit {
   typename Elem<T>::V8 r[4];
   // Tokens row .. row + 3 of a head at base, head elements d .. d + 7.  valid: bit i = token row + i counts (others become
-  // zero); rows: tokens that exist (>= 1); whole: uniform, all of the tile counts and vec holds.  With 16-byte loads every lane
-  // loads, absent tokens from the last one there is: no branches around loads.
+  // zero); rows: tokens that exist (>= 1); whole: uniform, all of the tile counts and vec holds.  Tokens that do not exist are never
+  // read: their place is taken by the last one there is.  With 16-byte loads every lane loads: no branches around loads.
   __device__ __forceinline__ void load(const T* base, long sl, int row, int rows, int d, int D, unsigned valid, bool vec,
                                        bool whole) {
     typedef typename Elem<T>::V8 V8;
@@ -95,7 +95,8 @@ struct Unit {
         if (d >= D || !((valid >> i) & 1)) r[i] = V8{};
     } else {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) r[i] = load8<T>(base + (long)(row + i) * sl + d, (valid >> i) & 1 ? D - d : 0, false);
+      for (int i = 0; i < 4; ++i)
+        r[i] = load8<T>(base + (long)min(row + i, rows - 1) * sl + d, (valid >> i) & 1 ? D - d : 0, false);
     }
   }
   template <int DP>
