@@ -3,6 +3,8 @@
 // wave (matrix instruction, shuffle, ballot, wave barrier) and goes on when the others have got there.  A launch is over when
 // hipLaunchKernelGGL returns.  Memory is the process's own, so a read out of range ends on a guard page (lanes.cpp).
 #pragma once
+#include <immintrin.h>
+
 #include <cmath>
 #include <cstddef>
 #include <cstdint>
@@ -80,6 +82,11 @@ template <typename V>
 Result mfma16(V a, V b, Result c) {
   return mfma<8>(a, b, c, [](const V& v, int s) { return (float)v[s]; });
 }
+typedef _Float16 Halves __attribute__((ext_vector_type(2)));
+inline Halves halves_towards_zero(float a, float b) {
+  const unsigned short h[2] = {_cvtss_sh(a, _MM_FROUND_TO_ZERO), _cvtss_sh(b, _MM_FROUND_TO_ZERO)};
+  return __builtin_bit_cast(Halves, h);
+}
 inline uint64_t ballot(bool on) {
   const char* all = wave_all(&on, sizeof on);
   uint64_t bits = 0;
@@ -95,6 +102,7 @@ inline uint64_t ballot(bool on) {
 #define __builtin_amdgcn_exp2f exp2f
 #define __builtin_amdgcn_logf log2f
 #define __builtin_amdgcn_rcpf(x) (1.f / (x))
+#define __builtin_amdgcn_cvt_pkrtz lanes::halves_towards_zero
 #define __builtin_amdgcn_readfirstlane(x) (x)                  // of values that are the same in every lane
 #define __builtin_amdgcn_inverse_ballot_w64(bits) ((((bits) >> (threadIdx.x & 63)) & 1) != 0)
 #define __builtin_amdgcn_mfma_f32_32x32x2f32(a, b, c, ...) lanes::mfma<1>(a, b, c, [](float v, int) { return v; })

@@ -124,34 +124,77 @@ __device__ __forceinline__ const typename Elem<T>::V8 frag_at(const T* tile, int
   return *reinterpret_cast<const typename Elem<T>::V8*>(tile + at);
 }
 
-// Registers 8c .. 8c + 7 of a 32x32 result as the second operand of the next product (16 of its 32 rows).  With T a 16-bit type,
-// the only rounding of P and dS: to the inputs' type, to nearest, as the matrix instruction takes no wider operand.  It adds as
-// much to the error of a result as its own rounding to the type does.
-template <typename T>
-__device__ __forceinline__ typename Elem<T>::V8 as_operand(const f32x16& s, int c) {
-  typename Elem<T>::V8 v;
+// Registers 8c .. 8c + 7 of a 32x32 result.
+__device__ __forceinline__ f32v8 part8(const f32x16& s, int c) {
+  f32v8 v;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) v[i] = (T)s[8 * c + i];
+  for (int i = 0; i < 8; ++i) v[i] = s[8 * c + i];
   return v;
 }
 
-// c += a b with b in fp32: 16-bit types take b as the sum of two operands, each rounded to the type, and so lose nothing of it
-// that their results could show.  For kernels whose matrix instructions are not what bounds them.
+// An fp32 value as the second operand of a product (P and dS): the matrix instructions of the 16-bit types take no wider one, so it is
+// the sum of two, and the product takes two instructions.  bf16 rounds both to nearest, fp16 towards zero (one instruction for two
+// elements): what is lost is at most 2^-16 or 2^-20 of the value, against the 2^-8 or 2^-11 of one operand, which would add as much to
+// the error of a result as its own rounding to the type does (long causal forward, bf16: 1.95e-3 of the result in all, with two
+// 1.52e-3).  All of a step's products take the first operand before the second: no two in a row add to the same registers.
 template <typename T>
-__device__ __forceinline__ f32x16 mma_wide(typename Elem<T>::V8 a, f32v8 b, f32x16 c) {
+struct Wide {
   typename Elem<T>::V8 high, low;
+  __device__ __forceinline__ explicit Wide(const f32v8& x);
+  // c[i] += frag(i) x
+  template <int N, typename F>
+  __device__ __forceinline__ void mma_all(f32x16 (&c)[N], F frag) const {
+    typename Elem<T>::V8 a[N];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    high[i] = (T)b[i];
-    low[i] = (T)(b[i] - (float)high[i]);
+    for (int i = 0; i < N; ++i) a[i] = frag(i);
+#pragma unroll
+    for (int i = 0; i < N; ++i) c[i] = Elem<T>::mma32(a[i], high, c[i]);
+#pragma unroll
+    for (int i = 0; i < N; ++i) c[i] = Elem<T>::mma32(a[i], low, c[i]);
   }
-  c = Elem<T>::mma32(a, high, c);
-  return Elem<T>::mma32(a, low, c);
+  __device__ __forceinline__ f32x16 mma(const typename Elem<T>::V8& a, f32x16 c) const {
+    return Elem<T>::mma32(a, low, Elem<T>::mma32(a, high, c));
+  }
+};
+template <>
+__device__ __forceinline__ Wide<__bf16>::Wide(const f32v8& x) {
+  struct {
+    bf16v2 pair[4];
+  } h, l;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const f32v2 v = {x[2 * i], x[2 * i + 1]};
+    h.pair[i] = __builtin_convertvector(v, bf16v2);
+    l.pair[i] = __builtin_convertvector((f32v2{v[0] - (float)h.pair[i][0], v[1] - (float)h.pair[i][1]}), bf16v2);
+  }
+  high = __builtin_bit_cast(bf16v8, h);
+  low = __builtin_bit_cast(bf16v8, l);
 }
 template <>
-__device__ __forceinline__ f32x16 mma_wide<float>(f32v8 a, f32v8 b, f32x16 c) {
-  return Elem<float>::mma32(a, b, c);
+__device__ __forceinline__ Wide<_Float16>::Wide(const f32v8& x) {
+  struct {
+    f16v2 pair[4];
+  } h, l;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    h.pair[i] = __builtin_bit_cast(f16v2, __builtin_amdgcn_cvt_pkrtz(x[2 * i], x[2 * i + 1]));
+    l.pair[i] = __builtin_bit_cast(
+        f16v2, __builtin_amdgcn_cvt_pkrtz(x[2 * i] - (float)h.pair[i][0], x[2 * i + 1] - (float)h.pair[i][1]));
+  }
+  high = __builtin_bit_cast(f16v8, h);
+  low = __builtin_bit_cast(f16v8, l);
 }
+template <>
+struct Wide<float> {
+  f32v8 x;
+  __device__ __forceinline__ explicit Wide(const f32v8& v) : x(v) {}
+  template <int N, typename F>
+  __device__ __forceinline__ void mma_all(f32x16 (&c)[N], F frag) const {
+#pragma unroll
+    for (int i = 0; i < N; ++i) c[i] = Elem<float>::mma32(frag(i), x, c[i]);
+  }
+  __device__ __forceinline__ f32x16 mma(const f32v8& a, f32x16 c) const { return Elem<float>::mma32(a, x, c); }
+};
 
 // fp16: P and dS are rounded as 16 P and 16 dS.  A row of n keys holds P of about 1 / n, which from n = 2^14 on, and dS sooner,
 // would fall among fp16's subnormals.  16 dS overflows where |dS| passes 4094, and |dS| is at most half the largest |dout . v|.
@@ -219,9 +262,9 @@ __device__ __forceinline__ void put_partial(const AttnArgs& a, long row, int spl
 
 // ---- forward ------------------------------------------------------------------------------------------------------
 // One workgroup = 32 NW queries of one head, one wave = 32 of them; the keys pass in tiles.  8192 tokens, 16 on 4 heads of 128,
-// bf16, causal: 338 us, 813 TFLOP/s, the matrix pipe busy 37 %; a wave reads 32 KB of LDS for each 32 x 64 scores, which
-// takes as long as their products, so what is left is in more queries a wave.  Two waves a SIMD (603 us at one) and loads
-// between the barriers, not a tile ahead in registers (which took a fifth more of them for the same time).
+// bf16, causal: 455 us, 907 TFLOP/s of its three products (P V takes two), where a large product reaches 1119 (331 us with P in one
+// operand, at the error told at Wide).  Two waves a SIMD (603 us at one, then) and loads between the barriers, not a tile ahead in
+// registers (which took a fifth more of them for the same time).
 // With few workgroups the tiles are cut into `splits` ranges, which attn_join_kernel joins.
 template <typename T, int DP, int NW>
 __global__ __launch_bounds__(NW * 64, sizeof(T) == 2 ? 2 : DP <= 64 ? 3 : 1) void attn_fwd_kernel(AttnArgs a) {
@@ -349,10 +392,8 @@ __global__ __launch_bounds__(NW * 64, sizeof(T) == 2 ? 2 : DP <= 64 ? 3 : 1) voi
     for (int t = 0; t < KT / 32; ++t)
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
-        const V8 p = as_operand<T>(s[t], c);
-#pragma unroll
-        for (int dt = 0; dt < ND; ++dt)
-          o[dt] = Elem<T>::mma32(frag_at<T>(vx, TileX<T, KT>::frag(dt * 32 + col, t * 2 + c, half)), p, o[dt]);
+        const Wide<T> p(part8(s[t], c));
+        p.mma_all(o, [&](int dt) { return frag_at<T>(vx, TileX<T, KT>::frag(dt * 32 + col, t * 2 + c, half)); });
       }
   }
   l += __shfl_xor(l, 32, 64);
@@ -481,10 +522,8 @@ __global__ __launch_bounds__(64) void attn_few_kernel(AttnArgs a) {
     }
 #pragma unroll
     for (int c = 0; c < 2; ++c) {
-      const f32v8 p = as_operand<float>(s, c);
-#pragma unroll
-      for (int dt = 0; dt < ND; ++dt)
-        o[dt] = mma_wide<T>(frag_at<T>(vx, TileX<T, KT>::frag(dt * 32 + col, c, half)), p, o[dt]);
+      const Wide<T> p(part8(s, c));
+      p.mma_all(o, [&](int dt) { return frag_at<T>(vx, TileX<T, KT>::frag(dt * 32 + col, c, half)); });
     }
   }
   l += __shfl_xor(l, 32, 64);
@@ -590,7 +629,8 @@ __global__ __launch_bounds__(256) void attn_join_rows_kernel(AttnArgs a) {
 // One workgroup = 32 NW queries of one head, keys in tiles of KT: S^T and dP^T = V dO^T share the layout of the forward,
 // dq^T += K^T dS^T.  delta = dout . out is formed here first and left for the dk / dv kernel.  With few workgroups the key tiles
 // are cut into `splits_q` shares, whose fp32 results attn_sum_q_kernel adds in order.  2 x 4001 tokens, 16 on 4 heads of 128,
-// bf16, causal: 345 us, 570 TFLOP/s of its three products (437 us with the next tile in registers, which spilled).
+// bf16, causal: 399 us, 660 TFLOP/s of its four products (dS K takes two); 350 us with dS in one operand.  The next tile in registers
+// spilled, and took a quarter longer.
 template <typename T, int DP, int NW>
 __global__ __launch_bounds__(NW * 64, sizeof(T) == 2 ? 2 : DP <= 32 ? 3 : DP <= 64 ? 2 : 1) void attn_dq_kernel(AttnArgs a) {
   typedef typename Elem<T>::V8 V8;
@@ -700,10 +740,8 @@ __global__ __launch_bounds__(NW * 64, sizeof(T) == 2 ? 2 : DP <= 32 ? 3 : DP <= 
       }
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
-        const V8 ds = as_operand<T>(s, c);
-#pragma unroll
-        for (int dt = 0; dt < ND; ++dt)
-          acc[dt] = Elem<T>::mma32(frag_at<T>(kx, TileX<T, KT>::frag(dt * 32 + col, t * 2 + c, half)), ds, acc[dt]);
+        const Wide<T> ds(part8(s, c));
+        ds.mma_all(acc, [&](int dt) { return frag_at<T>(kx, TileX<T, KT>::frag(dt * 32 + col, t * 2 + c, half)); });
       }
     }
   }
@@ -761,7 +799,8 @@ constexpr bool DKV_V_LDS = sizeof(T) == 2 && DP == 128;
 // One workgroup = 32 NW keys of one key head, one wave = 32 of them; the queries of every head that shares it pass in
 // tiles of 32.  S and dP = dO V^T here have queries as rows: dv^T += dO^T P, dk^T += Q^T dS.  The sums over heads
 // and queries stay in one accumulator in a fixed order: no atomics, the same bits every time.  2 x 4001 tokens, 16 on 4 heads
-// of 128, bf16, causal: 460 us, 570 TFLOP/s of its four products (1440 us without shares and at one wave a SIMD).
+// of 128, bf16, causal: 579 us, 680 TFLOP/s of its six products (dO P and Q dS take two); 470 us with P and dS in one operand, 1440 us
+// without shares and at one wave a SIMD.
 template <typename T, int DP, int NW>
 __global__ __launch_bounds__(NW * 64, sizeof(T) == 2 || DP <= 64 ? 2 : 1) void attn_dkv_kernel(AttnArgs a) {
   typedef typename Elem<T>::V8 V8;
@@ -876,33 +915,28 @@ __global__ __launch_bounds__(NW * 64, sizeof(T) == 2 || DP <= 64 ? 2 : 1) void a
       const V8 v = V_LDS ? frag_at<T>(vt, TileR<T, DP>::frag(wave * 32 + col, c, half)) : vf[V_LDS ? 0 : c];
       dp = Elem<T>::mma32(frag_at<T>(gt, TileR<T, DP>::frag(col, c, half)), v, dp);
     }
+    // 16 queries at a time: P and dS of the others take no operands' registers yet
 #pragma unroll
-    for (int g = 0; g < 4; ++g) {
-      const f32v4 ls = *reinterpret_cast<const f32v4*>(lse2s + 8 * g + 4 * half);
-      const f32v4 de = *reinterpret_cast<const f32v4*>(deltas + 8 * g + 4 * half);
+    for (int c = 0; c < 2; ++c) {
+      f32v8 p8, ds8;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int r = 4 * g + e;
-        float p = __builtin_amdgcn_exp2f(fmaf(s[r], a.scale_log2, -ls[e]));
-        float ds = p * (dp[r] - de[e]);
-        if (partial && 8 * g + e < sees_from) p = ds = 0.f;
-        s[r] = p;
-        dp[r] = ds;
+      for (int g = 2 * c; g < 2 * c + 2; ++g) {
+        const f32v4 ls = *reinterpret_cast<const f32v4*>(lse2s + 8 * g + 4 * half);
+        const f32v4 de = *reinterpret_cast<const f32v4*>(deltas + 8 * g + 4 * half);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int r = 4 * g + e;
+          float p = __builtin_amdgcn_exp2f(fmaf(s[r], a.scale_log2, -ls[e]));
+          float ds = p * (dp[r] - de[e]);
+          if (partial && 8 * g + e < sees_from) p = ds = 0.f;
+          p8[r - 8 * c] = p;
+          ds8[r - 8 * c] = ds;
+        }
       }
-    }
-#pragma unroll
-    for (int c = 0; c < 2; ++c) {
-      const V8 p = as_operand<T>(s, c);
-#pragma unroll
-      for (int dt = 0; dt < ND; ++dt)
-        dv[dt] = Elem<T>::mma32(frag_at<T>(gx, TileX<T, QT>::frag(dt * 32 + col, c, half)), p, dv[dt]);
-    }
-#pragma unroll
-    for (int c = 0; c < 2; ++c) {
-      const V8 ds = as_operand<T>(dp, c);
-#pragma unroll
-      for (int dt = 0; dt < ND; ++dt)
-        dk[dt] = Elem<T>::mma32(frag_at<T>(qx, TileX<T, QT>::frag(dt * 32 + col, c, half)), ds, dk[dt]);
+      const Wide<T> p(p8);
+      p.mma_all(dv, [&](int dt) { return frag_at<T>(gx, TileX<T, QT>::frag(dt * 32 + col, c, half)); });
+      const Wide<T> ds(ds8);
+      ds.mma_all(dk, [&](int dt) { return frag_at<T>(qx, TileX<T, QT>::frag(dt * 32 + col, c, half)); });
     }
   }
   if (j >= a.Lk) return;
@@ -1100,8 +1134,8 @@ __global__ __launch_bounds__(QB * KB * 64, (SHORT_WAVES<T, DP, QB, KB>)) void at
       if (KB * ND % NW == 0 || t < KB * ND) {
 #pragma unroll
         for (int c = 0; c < 2 * QB; ++c)
-          dv[n] = mma_wide<T>(frag_rows<T>(gt + c * 16 * S + t % ND * 32 + col, S, half),
-                              frag_rows<float>(xt + c * 16 * XS + t / ND * 32 + col, XS, half), dv[n]);
+          dv[n] = Wide<T>(frag_rows<float>(xt + c * 16 * XS + t / ND * 32 + col, XS, half))
+                      .mma(frag_rows<T>(gt + c * 16 * S + t % ND * 32 + col, S, half), dv[n]);
       }
     }
     __syncthreads();
@@ -1113,8 +1147,8 @@ __global__ __launch_bounds__(QB * KB * 64, (SHORT_WAVES<T, DP, QB, KB>)) void at
       if (KB * ND % NW == 0 || t < KB * ND) {
 #pragma unroll
         for (int c = 0; c < 2 * QB; ++c)
-          dk[n] = mma_wide<T>(frag_rows<T>(qt + c * 16 * S + t % ND * 32 + col, S, half),
-                              frag_rows<float>(xt + c * 16 * XS + t / ND * 32 + col, XS, half), dk[n]);
+          dk[n] = Wide<T>(frag_rows<float>(xt + c * 16 * XS + t / ND * 32 + col, XS, half))
+                      .mma(frag_rows<T>(qt + c * 16 * S + t % ND * 32 + col, S, half), dk[n]);
       }
     }
 #pragma unroll
@@ -1124,8 +1158,8 @@ __global__ __launch_bounds__(QB * KB * 64, (SHORT_WAVES<T, DP, QB, KB>)) void at
         f32x16 dq = {};
 #pragma unroll
         for (int c = 0; c < 2 * KB; ++c)
-          dq = mma_wide<T>(frag_rows<T>(kt + c * 16 * S + t % ND * 32 + col, S, half),
-                           frag_slots(xt + (t / ND * 32 + col) * XS + c * 16, half), dq);
+          dq = Wide<T>(frag_slots(xt + (t / ND * 32 + col) * XS + c * 16, half))
+                   .mma(frag_rows<T>(kt + c * 16 * S + t % ND * 32 + col, S, half), dq);
         const int row = t / ND * 32 + col;
         T* p = (T*)a.dq + b * a.vdq.sb + hq * a.vdq.sh + (long)row * a.vdq.sl;
 #pragma unroll
