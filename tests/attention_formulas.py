@@ -2,9 +2,10 @@
 leave one rounding to the type, that of the result: what is in between is held in 32 bits, or in two operands of 16.
 
 u = eps / 2 is half a step of the type, f = 2^-24.  A value taken as the sum of two 16-bit operands is off by w = 4 u^2 of itself at the
-most: the first rounding leaves a rest of 2 u (towards zero; u to nearest), of which the second loses as much again; fp16's second
-operand also ends at 2^-25, half its smallest number.  The rest as in tests/test_gpu_layers.py: D products in a score, n f for a sum of
-n terms, exp2 of a score that is off by e is off by the factor e."""
+most: the first rounding leaves a rest of 2 u (towards zero; u to nearest), of which the second loses as much again.  fp16's second
+operand has an end: its numbers are 2^-24 apart there, and rounding towards zero loses up to all of that (to nearest: half, 2^-25; that
+is what a result's own rounding loses).  The rest as in tests/test_gpu_layers.py: D products in a score, n f for a sum of n terms, exp2
+of a score that is off by e is off by the factor e."""
 import math
 
 import torch
@@ -23,6 +24,10 @@ def two(t):
 
 def tiny(t):
     return 2.0 ** -25 if t == torch.float16 else 2.0 ** -134
+
+
+def end(t):
+    return 2.0 ** -24 if t == torch.float16 else 2.0 ** -134
 
 
 def visible(B, Lq, Lk, device, causal=False, query_start=None, key_lengths=None, key_mask=None, **_):
@@ -68,7 +73,7 @@ def forward64(q, k, v, scale=None, **masks):
     some = torch.where(total == 0, 1.0, total)
     out = E / some @ V
     # a probability: its exponential and its operands; the sum: those of its terms
-    e_E = ((e + two(t)) * E + tiny(t) * see) / some
+    e_E = ((e + two(t)) * E + end(t) * see) / some
     e_total = ((e + Lk * F) * E).sum(-1, keepdim=True) / some
     err = SLACK * (e_E @ V.abs() + (e_total + (Lk + 4) * F) * (E / some @ V.abs())) + tiny(t)
     return {"out": (out.permute(0, 2, 1, 3), (half_step(t) * (out.abs() + err) + err).permute(0, 2, 1, 3))}
@@ -88,15 +93,17 @@ def backward64(dout, q, k, v, out, lse, scale=None, **masks):
     delta, e_delta = (dO * O).sum(-1, keepdim=True), D * F * (dO * O).abs().sum(-1, keepdim=True)
     dP, e_dP = dO @ _T(V), D * F * dO.abs() @ _T(V.abs())
     dS = P * (dP - delta)
-    # fp16 takes 16 P, and 16 dS or, where that would leave its range, dS times the power of two that brings a row's or column's
-    # largest to at least 2^13: the second operand's end is then 2^-25 / 2^13 of it
-    e_P = SLACK * (e + two(t) + 2 * F) * P + tiny(t) / 16 * see
+    # fp16 takes 16 P, and 16 dS or, where that would leave its range, dS times a power of two that brings the largest of those that share
+    # it to at least 2^14; the second operand's end is that of fp16 over that factor.  A head's (dq) or a sequence's (dk, and all of a short
+    # one) share no more than theirs
+    e_P = SLACK * (e + two(t) + 2 * F) * P + end(t) / 16 * see
     e_dS = SLACK * (P * (e_dP + e_delta) + (e + two(t) + 4 * F) * dS.abs())
-    end = tiny(t) * see
-    largest = (lambda d: torch.clamp(dS.abs().amax(d, keepdim=True) * 2.0 ** -13, min=2.0 ** -4)) if t == torch.float16 else (lambda d: 1.0)
+    def ends(d):
+        return end(t) * see * (torch.clamp(dS.abs().amax(d, keepdim=True) * 2.0 ** -14, min=2.0 ** -4) if t == torch.float16 else 1.0)
+
     fold = lambda x: x.view(B, Hk, G, Lk, D).sum(2)
     n = Lq * G
-    rows, columns = e_dS + end * largest(-1), e_dS + end * largest((1, 2) if t == torch.float16 else -2)
+    rows, columns = e_dS + ends((1, 2, 3) if Lq <= 64 and Lk <= 64 else (2, 3)), e_dS + ends((1, 2, 3))
     found = {}
     for name, val, err in (
             ("dq", scale * dS @ K, scale * (rows @ K.abs() + 2 * Lk * F * dS.abs() @ K.abs())),

@@ -10,7 +10,8 @@ import torch
 ROOT = os.path.dirname(os.path.dirname(os.path.dirname(os.path.abspath(__file__))))
 sys.path[:0] = [ROOT, os.path.join(ROOT, "tests")]
 
-import test_gpu_layers as formulas                        # the 64-bit formulas and their bounds
+import test_gpu_layers as formulas
+from attention_formulas import backward64, forward64
 from trace_amd import _cabi
 
 formulas.DEV = "cpu"
@@ -60,7 +61,7 @@ def run(lanes, case):
         t.copy_(torch.randn(shape, generator=g) * size)
         return t
 
-    q, k = filled((B, Lq, Hq, D)), filled((B, Lk, Hk, D))
+    q, k = filled((B, Lq, Hq, D), case.get("q", 1.0)), filled((B, Lk, Hk, D), case.get("k", 1.0))
     v, dout = filled((B, Lk, Hk, D), case.get("v", 1.0)), filled((B, Lq, Hq, D), case.get("dout", 1.0))
     masks = {"causal": case.get("causal", False)}
     start = lengths = mask = None
@@ -86,7 +87,8 @@ def run(lanes, case):
             lanes.call("trace_attention_backward", C.byref(desc), *map(at, (dout, q, k, v, out, lse, dq, dk, dv)), *work)
         else:
             lanes.call("trace_attention", C.byref(desc), *map(at, (q, k, v, out, lse)), *work)
-    want = formulas.attention64(q, k, v, dout, **masks)
+    want = {"lse": formulas.attention64(q, k, v, **masks)["lse"], **forward64(q, k, v, **masks),
+            **backward64(dout, q, k, v, out, lse, **masks)}
     for name, got in (("out", out), ("lse", lse), ("dq", dq), ("dk", dk), ("dv", dv)):
         formulas.near(got, *want[name], what=name)
 

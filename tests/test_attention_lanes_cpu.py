@@ -1,5 +1,5 @@
 """The attention kernels run lane by lane on the CPU (tests/lanes): every access stays within the tensors, which end at memory that may
-not be touched, and results are within the bounds of tests/test_gpu_layers.py."""
+not be touched, and results are within the bounds of attention_formulas.py."""
 import itertools
 import json
 import os
@@ -47,3 +47,11 @@ def test_accesses_stay_within_the_tensors(lanes, dtype):
         dict(size=[1, 65, 200, 1, 1, 72], key_lengths=[131]),
         dict(size=[1, 33, 1, 1, 1, 128]), dict(size=[2, 1, 90, 1, 1, 17]),
         dict(size=[3, 52, 52, 2, 1, 64], causal=True, masked=0.2)))])
+
+
+@pytest.mark.parametrize("size", [[1, 40, 40, 2, 1, 64], [1, 64, 20, 4, 1, 128], [2, 30, 33, 2, 2, 20], [1, 100, 70, 4, 2, 64],
+                                  [1, 65, 200, 2, 1, 128], [1, 20, 300, 1, 1, 32]])
+def test_large_fp16_gradients(lanes, size):
+    """dout of a scaled loss: dout . v far above what fp16 holds, gradients that it holds."""
+    run(lanes, [dict(dtype="f16", size=size, v=4.0, dout=1000.0),
+                dict(dtype="f16", size=size, v=8.0, dout=8000.0, q=0.05, k=0.01, causal=True)])

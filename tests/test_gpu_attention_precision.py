@@ -56,3 +56,35 @@ def test_one_rounding_of_single_tokens_in_cut_ranges(dtype, D, off):
     for Lq, Hq in ((1, 2), (1, 16), (4, 6)):
         q = torch.randn(B, Lq, Hq, D, generator=g, device=DEV).to(dtype)
         check(q, k, v, None, backward=False, key_lengths=lengths)
+
+
+@pytest.mark.parametrize("size", [(2, 40, 40, 2, 2, 64), (2, 30, 20, 4, 4, 128), (2, 24, 30, 4, 2, 128), (1, 64, 20, 4, 1, 128), (2, 52, 52, 4, 2, 32),
+                                  (2, 30, 33, 2, 2, 20), (1, 100, 70, 4, 2, 64), (1, 65, 900, 2, 1, 128), (40, 129, 200, 8, 8, 64)])
+@pytest.mark.parametrize("v, dout, qk, causal", [(4.0, 1000.0, 1.0, False), (8.0, 8000.0, 0.02, True), (1.0, 2.0 ** 12, 0.5, False),
+                                                 (1.0, 2.0 ** -10, 1.0, True)])
+def test_fp16_gradients_of_a_scaled_loss(size, v, dout, qk, causal):
+    """dout . v far above what fp16 holds (and far below 1), gradients that it holds: rows and heads of different sizes."""
+    q, k, w = inputs(torch.float16, *size)
+    d = inputs(torch.float16, *size, seed=3)[0].float() * dout
+    d = d * torch.linspace(0.1, 1, size[3], device=DEV)[:, None] * torch.linspace(1, 0.2, size[1], device=DEV)[:, None, None]
+    check(q * qk, k * qk, w * v, d.half(), causal=causal)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("size", [(1, 40, 40, 2, 2, 64), (1, 30, 20, 4, 4, 128), (1, 100, 170, 4, 2, 64)])
+def test_a_row_of_infinite_gradients_is_alone_in_dq(dtype, size):
+    """dout infinite in one row: the other rows' dq keep their bits (fp16's scale does not go by it)."""
+    q, k, v = inputs(dtype, *size)
+    dout = inputs(dtype, *size, seed=3)[0] * 100
+    out, lse = layers.attention(q, k, v)
+    want = layers.attention_backward(dout, q, k, v, out, lse)
+    dout[0, 7, 1] = float("inf")
+    got = layers.attention_backward(dout, q, k, v, out, lse)
+    assert not bool(torch.isfinite(got[0][0, 7, 1]).any())
+    other = torch.ones(size[1], size[3], dtype=torch.bool, device=DEV)
+    other[7, 1] = False
+    assert torch.equal(got[0][0][other], want[0][0][other])
+    heads = [h for h in range(size[4]) if h != 1 // (size[3] // size[4])]
+    for a, b in zip(got[1:], want[1:]):
+        assert torch.equal(a[:, :, heads], b[:, :, heads])
+        assert not bool(torch.isfinite(a[:, :, 1 // (size[3] // size[4])]).any())

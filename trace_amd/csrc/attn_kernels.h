@@ -196,8 +196,8 @@ struct Wide<float> {
   __device__ __forceinline__ f32x16 mma(const f32v8& a, f32x16 c) const { return Elem<float>::mma32(a, x, c); }
 };
 
-// fp16: P and dS are rounded as 16 P and 16 dS.  A row of n keys holds P of about 1 / n, which from n = 2^14 on, and dS sooner,
-// would fall among fp16's subnormals.  16 dS overflows where |dS| passes 4094, and |dS| is at most half the largest |dout . v|.
+// fp16: P and dS are taken as 16 P and 16 dS.  A row of n keys holds P of about 1 / n, which from n = 2^14 on, and dS sooner,
+// would fall among fp16's subnormals.
 template <typename T>
 constexpr float P_SHIFT = 0.f;
 template <>
@@ -206,6 +206,49 @@ template <typename T>
 constexpr float P_UNSHIFT = 1.f;
 template <>
 inline constexpr float P_UNSHIFT<_Float16> = 0.0625f;
+
+// |dS| is up to half the largest |dout . v| and so has no bound that fp16 could hold: where 16 dS passes FIT_LIMIT, a power of two
+// (`fit`, 1 until then, the same in all lanes of a wave) takes the largest down to 2^14 .. 2^15, and the sums so far with it.  The result
+// is divided by it again, in fp32.  The second operand then ends at 2^-38 of the largest.  All but a maximum and a
+// comparison is in the branch.
+template <typename T>
+constexpr bool FIT = false;
+template <>
+inline constexpr bool FIT<_Float16> = true;
+constexpr float FIT_LIMIT = 32768.f;
+__device__ __forceinline__ float fit_for(float most) {
+  return __builtin_bit_cast(float, (268u - ((__builtin_bit_cast(unsigned, most) >> 23) & 255u)) << 23);      // 2^(14 - exponent)
+}
+// The largest magnitude; zero if that is infinite: such a row's or column's results are lost, and others' scale must not go by it.
+template <typename V>
+__device__ __forceinline__ float most_of(const V& x) {
+  float m = 0.f;
+#pragma unroll
+  for (int i = 0; i < (int)(sizeof(V) / sizeof(float)); ++i) m = fmaxf(m, fabsf(x[i]));
+  return m < INFINITY ? m : 0.f;
+}
+__device__ __forceinline__ float wave_most(float m) {
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
+  return __builtin_bit_cast(float, __builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, m)));
+}
+// Makes the values ds of a step fit; acc holds sums of what came before.
+template <typename V, int N>
+__device__ __forceinline__ void make_fit(V& ds, f32x16 (&acc)[N], float& fit) {
+  const float most = most_of(ds);
+  if (__any(most * fit > FIT_LIMIT)) {
+    const float now = fit_for(wave_most(most));
+#pragma unroll
+    for (int n = 0; n < N; ++n)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) acc[n][r] *= now / fit;
+    fit = now;
+  }
+  if (fit != 1.f) {
+#pragma unroll
+    for (int i = 0; i < (int)(sizeof(V) / sizeof(float)); ++i) ds[i] *= fit;
+  }
+}
 
 // One bit per key of the tile at key0: below the sequence's length and not masked.  The same in every wave.
 __device__ __forceinline__ unsigned long long key_bits(const AttnArgs& a, int b, int key0, int len) {
@@ -709,6 +752,7 @@ __global__ __launch_bounds__(NW * 64, sizeof(T) == 2 ? 2 : DP <= 32 ? 3 : DP <= 
     }
   };
   f32x16 acc[ND] = {};
+  float fit = 1.f;
   unsigned long long bits = key_bits(a, b, from, end) & FULL;
   for (int key0 = from; key0 < stop; key0 += KT) {
     const unsigned long long here = bits;
@@ -738,6 +782,7 @@ __global__ __launch_bounds__(NW * 64, sizeof(T) == 2 ? 2 : DP <= 32 ? 3 : DP <= 
         for (int r = 0; r < 16; ++r)
           if (t * 32 + 8 * (r / 4) + r % 4 > room) s[r] = 0.f;
       }
+      if (FIT<T>) make_fit(s, acc, fit);
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
         const Wide<T> ds(part8(s, c));
@@ -746,6 +791,7 @@ __global__ __launch_bounds__(NW * 64, sizeof(T) == 2 ? 2 : DP <= 32 ? 3 : DP <= 
     }
   }
   if (i >= a.Lq) return;
+  const float unfit = FIT<T> ? 1.f / fit : 1.f;
   if (a.splits_q > 1) {
     float* p = a.part_q + (split * ((long)a.B * a.Hq * a.Lq) + row) * DP;
 #pragma unroll
@@ -753,10 +799,10 @@ __global__ __launch_bounds__(NW * 64, sizeof(T) == 2 ? 2 : DP <= 32 ? 3 : DP <= 
 #pragma unroll
       for (int g = 0; g < 4; ++g)
         *reinterpret_cast<f32v4*>(p + dt * 32 + g * 8 + half * 4) =
-            f32v4{acc[dt][4 * g], acc[dt][4 * g + 1], acc[dt][4 * g + 2], acc[dt][4 * g + 3]};
+            f32v4{acc[dt][4 * g] * unfit, acc[dt][4 * g + 1] * unfit, acc[dt][4 * g + 2] * unfit, acc[dt][4 * g + 3] * unfit};
     return;
   }
-  const float back = a.scale * P_UNSHIFT<T>;
+  const float back = a.scale * P_UNSHIFT<T> * unfit;
   T* p = (T*)a.dq + b * a.vdq.sb + hq * a.vdq.sh + (long)i * a.vdq.sl;
 #pragma unroll
   for (int dt = 0; dt < ND; ++dt)
@@ -846,6 +892,7 @@ __global__ __launch_bounds__(NW * 64, sizeof(T) == 2 || DP <= 64 ? 2 : 1) void a
   const long list = (long)per_head * a.G;
   const int begin = (int)(list * split / a.splits), total = (int)(list * (split + 1) / a.splits) - begin;
   f32x16 dk[ND] = {}, dv[ND] = {};
+  float fit = 1.f;
   const bool whole = vec && a.D == DP && 2 * UN % NT == 0;
   auto load_unit = [&](Unit<T>& to, float (&seen)[4], int n, int hq, int q0) {
     const int u = tid + n * NT;
@@ -935,11 +982,13 @@ __global__ __launch_bounds__(NW * 64, sizeof(T) == 2 || DP <= 64 ? 2 : 1) void a
       }
       const Wide<T> p(p8);
       p.mma_all(dv, [&](int dt) { return frag_at<T>(gx, TileX<T, QT>::frag(dt * 32 + col, c, half)); });
+      if (FIT<T>) make_fit(ds8, dk, fit);
       const Wide<T> ds(ds8);
       ds.mma_all(dk, [&](int dt) { return frag_at<T>(qx, TileX<T, QT>::frag(dt * 32 + col, c, half)); });
     }
   }
   if (j >= a.Lk) return;
+  const float unfit = FIT<T> ? 1.f / fit : 1.f;
   if (a.splits > 1) {
     const long rows = (long)a.B * a.Hk * a.Lk, row = ((long)b * a.Hk + hk) * a.Lk + j;
     float* pk = a.part_o + (2 * split * rows + row) * DP;
@@ -949,12 +998,13 @@ __global__ __launch_bounds__(NW * 64, sizeof(T) == 2 || DP <= 64 ? 2 : 1) void a
 #pragma unroll
       for (int g = 0; g < 4; ++g) {
         const int d = dt * 32 + g * 8 + half * 4;
-        *reinterpret_cast<f32v4*>(pk + d) = f32v4{dk[dt][4 * g], dk[dt][4 * g + 1], dk[dt][4 * g + 2], dk[dt][4 * g + 3]};
+        *reinterpret_cast<f32v4*>(pk + d) =
+            f32v4{dk[dt][4 * g] * unfit, dk[dt][4 * g + 1] * unfit, dk[dt][4 * g + 2] * unfit, dk[dt][4 * g + 3] * unfit};
         *reinterpret_cast<f32v4*>(pv + d) = f32v4{dv[dt][4 * g], dv[dt][4 * g + 1], dv[dt][4 * g + 2], dv[dt][4 * g + 3]};
       }
     return;
   }
-  const float back = a.scale * P_UNSHIFT<T>;
+  const float back = a.scale * P_UNSHIFT<T> * unfit;
   T* pk = (T*)a.dk + b * a.vdk.sb + hk * a.vdk.sh + (long)j * a.vdk.sl;
   T* pv = (T*)a.dv + b * a.vdv.sb + hk * a.vdv.sh + (long)j * a.vdv.sl;
 #pragma unroll
@@ -1002,7 +1052,9 @@ __device__ __forceinline__ typename Elem<T>::V8 frag_rows(const T* p, int stride
 template <typename T, int DP, int QB, int KB>
 constexpr int SHORT_WAVES = sizeof(T) == 2 ? (DP == 32 ? 3 : DP == 64 ? 2 : 1) : (DP == 32 || (DP == 64 && QB * KB == 4) ? 2 : 1);
 
-template <typename T, int DP, int QB, int KB>
+// MANY: where dS has to be made fit, the sums of other heads may have to as well.  (It takes registers: fp16, 4096 sequences of 30 on
+// 4 heads of 128: 332 us without, 445 with.)
+template <typename T, int DP, int QB, int KB, bool MANY>
 __global__ __launch_bounds__(QB * KB * 64, (SHORT_WAVES<T, DP, QB, KB>)) void attn_short_backward_kernel(AttnArgs a) {
   typedef typename Elem<T>::V8 V8;
   constexpr int NW = QB * KB, NT = NW * 64, NC = DP / 16, ND = DP / 32, S = TileN<T, DP>::S, XS = TileN<float, 32 * KB>::S;
@@ -1013,6 +1065,7 @@ __global__ __launch_bounds__(QB * KB * 64, (SHORT_WAVES<T, DP, QB, KB>)) void at
   T* const gt = qt + 32 * QB * S;
   T* const kt = gt + 32 * QB * S;
   float* const xt = reinterpret_cast<float*>(kt + 32 * KB * S);          // P, then dS: (query, key)
+  float* const most_s = xt + 32 * QB * XS;                               // FIT: of each wave, what passes the limit
   const long item = xcd_item(a.items);
   if (item >= a.items) return;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, col = lane & 31, half = lane >> 5;
@@ -1042,7 +1095,7 @@ __global__ __launch_bounds__(QB * KB * 64, (SHORT_WAVES<T, DP, QB, KB>)) void at
     }
   }
   f32x16 dk[KTILES] = {}, dv[KTILES] = {};
-  const float back = a.scale * P_UNSHIFT<T>;
+  float fit = 1.f;                                                       // the same in every wave
   for (int g = 0; g < a.G; ++g) {
     const int hq = hk * a.G + g;
     const float* lse_row = a.lse_in + ((long)b * a.Hq + hq) * a.Lq;
@@ -1125,6 +1178,11 @@ __global__ __launch_bounds__(QB * KB * 64, (SHORT_WAVES<T, DP, QB, KB>)) void at
       for (int q = 0; q < 4; ++q)
         *reinterpret_cast<f32v4*>(xt + i * XS + ki * 32 + 8 * q + 4 * half) = f32v4{x[4 * q], x[4 * q + 1], x[4 * q + 2], x[4 * q + 3]};
     };
+    if (FIT<T>) {
+      float most = most_of(dp);
+      if (__any(most * fit > FIT_LIMIT)) most = wave_most(most);
+      if (lane == 0) most_s[wave] = most;
+    }
     // tile t of a gradient: token block t / ND, head elements 32 (t % ND) .. + 31
     put(s);
     __syncthreads();
@@ -1138,6 +1196,26 @@ __global__ __launch_bounds__(QB * KB * 64, (SHORT_WAVES<T, DP, QB, KB>)) void at
                       .mma(frag_rows<T>(gt + c * 16 * S + t % ND * 32 + col, S, half), dv[n]);
       }
     }
+    if (FIT<T>) {
+      float most = most_s[0];
+#pragma unroll
+      for (int w = 1; w < NW; ++w) most = fmaxf(most, most_s[w]);
+      if (most * fit > FIT_LIMIT) {
+        const float now = fit_for(most);
+        if (MANY) {
+#pragma unroll
+          for (int n = 0; n < KTILES; ++n)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) dk[n][r] *= now / fit;
+        }
+        fit = now;
+      }
+      if (fit != 1.f) {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) dp[r] *= fit;
+      }
+    }
+    const float back = a.scale * P_UNSHIFT<T> / fit;
     __syncthreads();
     put(dp);
     __syncthreads();
@@ -1172,6 +1250,7 @@ __global__ __launch_bounds__(QB * KB * 64, (SHORT_WAVES<T, DP, QB, KB>)) void at
       }
     }
   }
+  const float back = a.scale * P_UNSHIFT<T> / fit;
 #pragma unroll
   for (int n = 0; n < KTILES; ++n) {
     const int t = wave + n * NW, row = t / ND * 32 + col;

@@ -72,12 +72,17 @@ int dkv(AttnArgs a, hipStream_t st) {
   return launch_status("attn_sum_kernel");
 }
 
-template <typename T, int DP, int QB, int KB>
-int short_backward(AttnArgs a, hipStream_t st) {
+template <typename T, int DP, int QB, int KB, bool MANY>
+int short_heads(AttnArgs a, hipStream_t st) {
   static unsigned long long attr = 0;
   a.items = (long)a.Hk * a.B;
-  const size_t lds = sizeof(T) * (2 * QB + KB) * 32 * TileN<T, DP>::S + sizeof(float) * 32 * QB * TileN<float, 32 * KB>::S;
-  return launch(&attn_short_backward_kernel<T, DP, QB, KB>, &attr, lds, QB * KB * 64, a, st, "attn_short_backward_kernel");
+  const size_t lds = sizeof(T) * (2 * QB + KB) * 32 * TileN<T, DP>::S + sizeof(float) * 32 * QB * TileN<float, 32 * KB>::S +
+                     (FIT<T> ? sizeof(float) * QB * KB : 0);
+  return launch(&attn_short_backward_kernel<T, DP, QB, KB, MANY>, &attr, lds, QB * KB * 64, a, st, "attn_short_backward_kernel");
+}
+template <typename T, int DP, int QB, int KB>
+int short_backward(const AttnArgs& a, hipStream_t st) {
+  return FIT<T> && a.G > 1 ? short_heads<T, DP, QB, KB, FIT<T>>(a, st) : short_heads<T, DP, QB, KB, false>(a, st);
 }
 template <typename T, int DP>
 int short_blocks(const AttnArgs& a, hipStream_t st) {
