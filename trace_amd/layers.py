@@ -11,6 +11,7 @@ import ctypes as C
 import math
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _cabi
 
@@ -24,13 +25,15 @@ def _refuse(text, *args):
 
 def _check(name, t, dtype=None, device=None, shape=None, dims=None):
     """Refuses what a kernel cannot take: another type (dtype None: one of the three), device or shape, an innermost
-    dimension that is not contiguous, a tensor that autograd would have to record.  (Plain ifs: a small call is bound by its
-    time on the host.)"""
+    dimension that is not contiguous, a tensor that autograd would have to record or carry a tangent on for.  (Plain ifs: a small
+    call is bound by its time on the host.)"""
     if not isinstance(t, torch.Tensor):
         _refuse("%s must be a tensor", name)
     if t.requires_grad and torch.is_grad_enabled():
         _refuse("%s requires grad: these operators record nothing for autograd; call them under torch.no_grad() and use "
                 "their backward functions", name)
+    if forward_ad._current_level >= 0 and forward_ad.unpack_dual(t).tangent is not None:       # a level: kept cheap outside of one
+        _refuse("%s has a forward-mode tangent, which these operators do not carry on", name)
     if dtype is None:
         if t.dtype not in _DTYPES:
             _refuse("%s has type %s (float32, bfloat16 or float16)", name, t.dtype)
