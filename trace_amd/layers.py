@@ -245,6 +245,10 @@ def rotary(q, positions, freqs, k=None, interleaved=False, scale=1.0, inverse=Fa
                             *(none if k is None else ok.stride()[:3]))
     _enqueue("trace_rotary", q.device, C.byref(desc), q.data_ptr(), _at(k), positions.data_ptr(), freqs.data_ptr(),
              oq.data_ptr(), _at(ok))
+    if inplace:
+        for t in (q, k):
+            if t is not None and not t.is_inference():
+                torch.autograd.graph.increment_version(t)        # who saved it for a backward pass is told there
     return oq if k is None else (oq, ok)
 
 
