@@ -6,6 +6,7 @@
 // 2 x 8192 tokens, 32 + 8 heads of 128, bf16: 66 us, 5.1 TB/s; 532480 tokens, 4 + 4 heads of 64, fp32: 421 us, 5.2 TB/s.
 #include "layer_types.h"
 
+#include <algorithm>
 #include <cmath>
 
 namespace trace {
@@ -162,8 +163,9 @@ extern "C" int trace_rotary(const trace_rotary_desc* d, const void* q, const voi
   a.tokens = (long)d->B * d->L;
   a.scale = d->scale;
   a.sin_sign = d->inverse ? -1.f : 1.f;
-  // a sine for each lane, or one token
-  a.per_wg = a.half >= 256 ? 1 : 256 / a.half;
+  // a sine for each lane, or one token; and no more elements than a workgroup's 32-bit index counts, 256 lanes further included
+  const int64_t most = (1 << 30) / ((int64_t)a.H * d->D);         // 16 or more
+  a.per_wg = a.half >= 256 ? 1 : (int)std::min<int64_t>(256 / a.half, most);
   const long grid = (a.tokens + a.per_wg - 1) / a.per_wg;
   TRACE_REQUIRE(grid * 256 <= MAX_GRID_THREADS, "trace_rotary: grid of %ld workgroups", grid);
   const size_t lds = (size_t)a.per_wg * a.half * sizeof(float2);
