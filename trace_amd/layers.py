@@ -32,7 +32,7 @@ def _check(name, t, dtype=None, device=None, shape=None, dims=None):
     if t.requires_grad and torch.is_grad_enabled():
         _refuse("%s requires grad: these operators record nothing for autograd; call them under torch.no_grad() and use "
                 "their backward functions", name)
-    if forward_ad._current_level >= 0 and forward_ad.unpack_dual(t).tangent is not None:       # a level: kept cheap outside of one
+    if forward_ad._current_level >= 0 and forward_ad.unpack_dual(t).tangent is not None:   # no level: no call
         _refuse("%s has a forward-mode tangent, which these operators do not carry on", name)
     if dtype is None:
         if t.dtype not in _DTYPES:
@@ -201,12 +201,50 @@ def rotary_frequencies(rot, base=10000.0, scaling="none", factor=1.0, trained_le
     return f.to(device), scale
 
 
+def _extent(t):
+    """Elements from the first of t to behind the last."""
+    return 1 + sum((n - 1) * s for n, s in zip(t.shape, t.stride())) if t.numel() else 0
+
+
+def _folds(t):
+    """Whether two elements of t may be the same memory: a dimension that does not reach over those within it."""
+    reach = 1
+    for s, n in sorted((s, n) for s, n in zip(t.stride(), t.shape) if n > 1) if t.numel() else ():
+        if s < reach:
+            return True
+        reach += (n - 1) * s
+    return False
+
+
+def _share(q, k):
+    """Whether q and k (B, L, heads, D), neither of which folds, have an element in common.  Windows of one layout: whether their
+    distance is a sum of strides, as often as indices can differ; other pairs count as sharing what they both reach over."""
+    size, apart = q.element_size(), k.data_ptr() - q.data_ptr()
+    if not (q.numel() and k.numel() and -_extent(k) * size < apart < _extent(q) * size):
+        return False
+    steps = []
+    for sq, nq, sk, nk in zip(q.stride(), q.shape, k.stride(), k.shape):
+        if nq > 1 and nk > 1 and sq != sk or apart % size:
+            return True
+        if nq > 1 or nk > 1:
+            steps.append((sq if nq > 1 else sk, 1 - nk, nq - 1))
+
+    def meet(rest, steps):
+        if not steps:
+            return rest == 0
+        s, low, high = steps[0]
+        return any(low <= d <= high and meet(rest - d * s, steps[1:]) for d in (rest // s, rest // s + 1))
+
+    return meet(apart // size, sorted(steps, reverse=True))
+
+
 def rotary(q, positions, freqs, k=None, interleaved=False, scale=1.0, inverse=False, inplace=False):
     """Rotates the first 2 len(freqs) elements of every head of q (B, L, Hq, D), and of k (B, L, Hk, D), by their
     positions: pair (a, b) number p at position t becomes scale (a cos w - b sin w, b cos w + a sin w), w = t freqs[p],
     angles in 64 bits.  Pairs are the two halves' elements p, or elements 2p, 2p + 1 if interleaved.  inverse: -w, which
     is also the gradient (of the same scale).  positions (L) or (B, L), int32 or int64, of any sign; freqs float64.
-    inplace: the results replace q and k.  Returns the rotated q, or (q, k)."""
+    inplace: the results replace q and k, which may be windows of one tensor but share no element.  Returns the rotated q, or
+    (q, k)."""
     _check("q", q, dims=4)
     device = q.device
     B, L, Hq, D = q.shape
@@ -227,13 +265,10 @@ def rotary(q, positions, freqs, k=None, interleaved=False, scale=1.0, inverse=Fa
         _refuse("scale is not finite")
     if inplace:
         for name, t in (("q", q), ("k", k)):
-            if t is not None and any(s == 0 and n > 1 for s, n in zip(t.stride(), t.shape)):
-                _refuse("%s is broadcast: it cannot be rotated in place", name)
-        if k is not None and q.stride() == k.stride():
-            # windows of one layout: apart by their heads, or side by side within a head's stride
-            head, apart = q.stride(2), (k.data_ptr() - q.data_ptr()) // q.element_size()
-            if -k.shape[2] * head < apart < Hq * head and not D <= apart % head <= head - D and q.numel() and k.numel():
-                _refuse("q and k share memory: they cannot be rotated in place together")
+            if t is not None and _folds(t):
+                _refuse("%s is broadcast or overlaps itself: it cannot be rotated in place", name)
+        if k is not None and _share(q, k):
+            _refuse("q and k share memory: they cannot be rotated in place together")
     _gpu(q)
     oq = q if inplace else torch.empty(q.shape, dtype=q.dtype, device=q.device)
     ok = k if k is None or inplace else torch.empty(k.shape, dtype=k.dtype, device=k.device)
