@@ -252,7 +252,7 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void residual_norm_backward_
         }
 #pragma unroll
         for (int e = 0; e < V; ++e) o[e] = a.y ? a.alpha * d[k][e] : d[k][e];
-        if (a.dx) row_store<TX, V>((TX*)a.dx + row * a.C + c, o);
+        row_store<TX, V>((TX*)a.dx + row * a.C + c, o);
         if (!a.y) continue;
         if (a.gate) row_load<float, V>(w, a.gate + gtab + c, true);
         if (a.post) row_load<float, V>(p, a.post + c, true);

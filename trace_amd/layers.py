@@ -338,8 +338,8 @@ def _norm_desc(x, y, gate, post_weight, weight, bias, kind, residual_scale, eps,
     per = min(rows_per_cond or max(rows, 1), max(rows, 1))
     groups = -(-rows // per) if rows else 1
     gate_cond = gate is not None and _table("gate", gate, device, groups, columns)
-    if post_weight is not None and (_table("post_weight", post_weight, device, 1, columns)):
-        _refuse("post_weight has one row")
+    if post_weight is not None:
+        _table("post_weight", post_weight, device, 1, columns)
     w_cond = weight is not None and _table("weight", weight, device, groups, columns)
     b_cond = bias is not None and _table("bias", bias, device, groups, columns)
     if weight is not None and bias is not None and w_cond != b_cond:
