@@ -402,7 +402,8 @@ typedef struct {
 /* Attention of q (B, Lq, Hq, D) over k, v (B, Lk, Hk, D); heads hq of q share key head hq / (Hq / Hk).
  * Query i of sequence b sees key j iff  j < key_lengths[b]  and  key_mask[b, j] != 0  and, if causal,
  * j <= i + query_start[b].  Keys that no length or mask admits are not read into any result, whatever they hold (NaN
- * included); of keys that only causality hides from a query this holds as long as they are finite. */
+ * included); of keys that only causality hides from a query this holds as long as they are finite.  Results that an infinite
+ * value, or dout, of a visible pair enters are infinite or NaN. */
 typedef struct {
   int dtype;
   int B, Lq, Lk, Hq, Hk, D;           /* Hq % Hk == 0, 1 <= D <= 128 */

@@ -106,9 +106,11 @@ struct BackPlan {
   int64_t part_g, part_s;         // floats of one partial table
 };
 
-// Rows are cut into chunks of one conditioning group each, for 16 waves a CU (eight where a row takes 1024 lanes): the column sums
-// fill the registers of four waves a SIMD.  Four times as many measured 2 % faster for 10240 groups and leave four times as many
-// partial rows to add up; twice as many were 15 % slower (a second, partly filled round).
+// Rows are cut into chunks of one conditioning group each, for the 16 waves a CU that the registers of the column sums leave room for
+// (four a SIMD); rows of 1024 lanes for two workgroups a CU, of which one runs at a time.  Up to 4096 columns, four times as many
+// measured 2 % faster for 10240 groups and leave four times as many partial rows to add up; twice as many were 15 % slower (a second,
+// partly filled round).  A lane of a 1024-lane row has 128 registers, and 16 elements of every array do not fit: 4096 x 16384 fp32 take
+// 971 us (1.7 TB/s, 380 .. 700 bytes of scratch a lane), where 8192 x 8192, eight a lane, take 407 (4.0 TB/s).
 BackPlan back_plan(const trace_norm_desc& d, int tpr, int teams_wg) {
   BackPlan b;
   const int target = tpr == 64 ? 4096 : tpr == 256 ? 1024 : 512;

@@ -126,7 +126,7 @@ def attention(q, k, v, causal=False, query_start=None, key_lengths=None, key_mas
     Query i sees key j iff j < key_lengths[b] (int32), key_mask[b, j] (bool) and, if causal, j <= i + query_start[b]
     (int32; None: the last query is at the last key, Lk - Lq).  For one new token a sequence on a cache: Lq = 1 and
     key_lengths.  Keys that no length or mask admits may hold anything, NaN included; keys that only causality hides
-    from some queries have to be finite.
+    from some queries have to be finite.  Results that an infinite value enters are infinite or NaN.
 
     Returns out (B, Lq, Hq, D) and lse (B, Hq, Lq) fp32, the log of the softmax's denominator: what attention_backward
     needs.  A query that sees no key gets 0 and -inf."""
