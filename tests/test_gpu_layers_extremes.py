@@ -77,3 +77,14 @@ def test_gradients_of_long_rows(dtype, size):
     want = backward64(dout, q, k, v, out, lse)
     for name, got in zip(("dq", "dk", "dv"), layers.attention_backward(dout, q, k, v, out, lse)):
         near(got, *want[name], what=name)
+
+
+def test_residual_norm_gradient_of_the_most_rows():
+    """2^31 - 1 rows of one element, one group: without dz the gradient of x is dh."""
+    dh = torch.empty(2 ** 31 - 1, 1, dtype=torch.bfloat16, device=DEV)
+    part = torch.randn(2 ** 24 + 3, device=DEV, generator=torch.Generator(DEV).manual_seed(1)).to(dh.dtype)
+    for at in range(0, dh.shape[0], part.shape[0]):
+        n = min(part.shape[0], dh.shape[0] - at)
+        dh[at:at + n, 0] = part[:n]
+    got = layers.residual_norm_backward(dh, None, dh)
+    assert torch.equal(got["dx"], dh) and got["dy"] is None

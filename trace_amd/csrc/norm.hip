@@ -114,17 +114,19 @@ struct BackPlan {
 BackPlan back_plan(const trace_norm_desc& d, int tpr, int teams_wg) {
   BackPlan b;
   const int target = tpr == 64 ? 4096 : tpr == 256 ? 1024 : 512;
-  b.groups = (int)(((int64_t)d.rows + d.rows_per_cond - 1) / d.rows_per_cond);
-  const int rpc = d.rows_per_cond < d.rows ? d.rows_per_cond : d.rows;
-  int nsub = target / b.groups;
-  const int most = (rpc + 1) / 2;                            // two rows at least: with few rows it is a team's rows one by one that take the time
-  nsub = nsub < 1 ? 1 : nsub > most ? most : nsub;
-  b.rows_sub = (rpc + nsub - 1) / nsub;
-  b.nsub = (rpc + b.rows_sub - 1) / b.rows_sub;
-  b.chunks = b.groups * b.nsub;
-  const int teams = b.chunks < target ? b.chunks : target;
-  b.per_team = (b.chunks + teams - 1) / teams;
-  b.teams = (b.chunks + b.per_team - 1) / b.per_team;
+  const int64_t rpc = d.rows_per_cond < d.rows ? d.rows_per_cond : d.rows;         // up to 2^31 - 1, as the rows
+  const int64_t groups = (d.rows + rpc - 1) / rpc;
+  const int64_t most = (rpc + 1) / 2;                        // two rows at least: with few rows it is a team's rows one by one that take the time
+  const int64_t cut = std::max<int64_t>(1, std::min(target / groups, most));
+  const int64_t rows_sub = (rpc + cut - 1) / cut, nsub = (rpc + rows_sub - 1) / rows_sub;
+  const int64_t chunks = groups * nsub, teams = std::min<int64_t>(chunks, target);
+  const int64_t per_team = (chunks + teams - 1) / teams;
+  b.groups = (int)groups;
+  b.rows_sub = (int)rows_sub;
+  b.nsub = (int)nsub;
+  b.chunks = (int)chunks;
+  b.per_team = (int)per_team;
+  b.teams = (int)((chunks + per_team - 1) / per_team);
   b.wgs = (b.teams + teams_wg - 1) / teams_wg;
   b.part_g = b.nsub > 1 && (d.per_cond || d.gate_per_cond) ? (int64_t)b.chunks * d.C : 0;
   b.part_s = (int64_t)b.wgs * d.C;

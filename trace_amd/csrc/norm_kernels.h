@@ -182,7 +182,7 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void residual_norm_backward_
     const int g = chunk / a.nsub, sub = chunk % a.nsub;
     const long base = (long)g * a.rpc;
     const int r0 = sub * a.rows_sub;
-    const int r1 = (int)min((long)min(r0 + a.rows_sub, a.rpc), a.R - base);
+    const int r1 = (int)min(min((long)r0 + a.rows_sub, (long)a.rpc), a.R - base);
     const long tab = a.cond ? (long)g * a.C : 0, gtab = a.gate_cond ? (long)g * a.C : 0;
     for (int r = r0; r < r1; ++r) {
       const long row = base + r;
