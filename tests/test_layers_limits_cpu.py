@@ -23,3 +23,16 @@ def test_norm_workspace_of_the_most_rows(columns, waves, rows, per, cond):
     assert 0 < n <= 4 * columns * (4 * (waves // teams + 1) + 3 * most * cond)
     if groups < waves // 2:                               # enough chunks for every team, give or take a rounding
         assert n >= 4 * columns * 4 * (waves // teams) // 2
+
+
+def test_attention_backward_refuses_more_query_tiles_than_it_counts():
+    """Tiles of 32 queries of the heads that share a key head, counted in 32 bits; the forward pass has no such count."""
+    L = _cabi.lib()
+    for Lq, Hq, Hk, ok in ((2 ** 30, 64, 1, False), (2 ** 30, 64, 2, True), (2 ** 30, 128, 2, False), (2 ** 20, 2 ** 16, 1, False),
+                           (2 ** 20, 65535, 1, True)):
+        d = _cabi.AttentionDesc(0, 1, Lq, 1, Hq, Hk, 1, 1.0)
+        got = [L.trace_attention_workspace_bytes(C.byref(d), b) for b in (0, 1)]
+        assert got[0] >= 0 and (got[1] >= 0) == ok, (Lq, Hq, Hk)
+        if not ok:
+            assert got[1] == -1 and "tiles" in L.trace_last_error().decode()
+            assert L.trace_attention_backward(C.byref(d), *[None] * 10, 0, None) == -1 and "tiles" in L.trace_last_error().decode()

@@ -34,6 +34,14 @@ int check_desc(const trace_attention_desc* d, const char* who) {
   return TRACE_OK;
 }
 
+int check_back(const trace_attention_desc* d, const char* who) {
+  const int rc = check_desc(d, who);
+  if (rc != TRACE_OK) return rc;
+  // attn_dkv_kernel counts the query tiles of the heads that share a key head in 32 bits
+  TRACE_REQUIRE(((int64_t)d->Lq + 31) / 32 * (d->Hq / d->Hk) < (1ll << 31), "%s: more than 2^31 tiles of 32 queries to a key head", who);
+  return TRACE_OK;
+}
+
 AttnArgs common_args(const trace_attention_desc& d) {
   AttnArgs a{};
   a.B = d.B; a.Lq = d.Lq; a.Lk = d.Lk; a.Hq = d.Hq; a.Hk = d.Hk; a.G = d.Hq / d.Hk; a.D = d.D;
@@ -119,7 +127,7 @@ int by_type(int dtype, AttnPass pass, const AttnArgs& a, hipStream_t st) {
 using namespace trace;
 
 extern "C" int64_t trace_attention_workspace_bytes(const trace_attention_desc* d, int backward) {
-  const int rc = check_desc(d, "trace_attention_workspace_bytes");
+  const int rc = backward ? check_back(d, "trace_attention_workspace_bytes") : check_desc(d, "trace_attention_workspace_bytes");
   if (rc != TRACE_OK) return rc;
   if (d->B == 0 || d->Lq == 0) return 0;
   return backward ? back_plan(*d).bytes : forward_plan(*d).bytes;
@@ -157,7 +165,7 @@ extern "C" int trace_attention(const trace_attention_desc* d, const void* q, con
 extern "C" int trace_attention_backward(const trace_attention_desc* d, const void* dout, const void* q, const void* k,
                                         const void* v, const void* out, const float* lse, void* dq, void* dk, void* dv,
                                         void* workspace, int64_t workspace_bytes, void* stream) {
-  const int rc = check_desc(d, "trace_attention_backward");
+  const int rc = check_back(d, "trace_attention_backward");
   if (rc != TRACE_OK) return rc;
   if (d->B == 0) return TRACE_OK;
   TRACE_REQUIRE((d->Lq == 0 || (dout && q && out && lse && dq)) && (d->Lk == 0 || (k && v && dk && dv)),
