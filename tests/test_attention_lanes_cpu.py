@@ -5,6 +5,7 @@ import json
 import os
 import subprocess
 import sys
+from concurrent.futures import ThreadPoolExecutor
 
 import pytest
 
@@ -19,10 +20,16 @@ def lanes(tmp_path_factory):
     return lanes_build.build(str(tmp_path_factory.mktemp("lanes")))
 
 
-def run(lanes, cases):
-    p = subprocess.run([sys.executable, os.path.join(HERE, "lanes", "attention.py"), lanes], capture_output=True, text=True,
-                       input="\n".join(json.dumps(c) for c in cases), timeout=600)
-    assert p.returncode == 0 and p.stdout.endswith("done\n"), p.stdout[-300:] + p.stderr[-2000:]
+def run(lanes, cases, at_once=4):
+    """The cases, dealt to a few processes; each ends at its first that fails, with the case's line as its last."""
+    cmd = [sys.executable, os.path.join(HERE, "lanes", "attention.py"), lanes]
+    jobs = [subprocess.Popen(cmd, stdin=subprocess.PIPE, stdout=subprocess.PIPE, stderr=subprocess.PIPE, text=True)
+            for _ in range(min(at_once, len(cases)))]
+    with ThreadPoolExecutor(len(jobs)) as pool:
+        said = list(pool.map(lambda n: jobs[n].communicate("\n".join(json.dumps(c) for c in cases[n::len(jobs)]), timeout=600),
+                             range(len(jobs))))
+    for job, (out, err) in zip(jobs, said):
+        assert job.returncode == 0 and out.endswith("done\n"), out[-300:] + err[-2000:]
 
 
 SHORT = ((1, 1), (1, 2), (31, 33), (32, 32), (33, 1), (33, 31), (64, 50), (2, 63), (63, 64))
