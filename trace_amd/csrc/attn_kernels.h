@@ -305,8 +305,9 @@ __device__ __forceinline__ void put_partial(const AttnArgs& a, long row, int spl
 
 // ---- forward ------------------------------------------------------------------------------------------------------
 // One workgroup = 32 NW queries of one head, one wave = 32 of them; the keys pass in tiles.  8192 tokens, 16 on 4 heads of 128,
-// bf16, causal: 455 us, 907 TFLOP/s of its three products (P V takes two), where a large product reaches 1119 (331 us with P in one
-// operand, at the error told at Wide).  Two waves a SIMD (603 us at one, then) and loads between the barriers, not a tile ahead in
+// bf16, causal: 427 .. 455 us, 907 .. 966 TFLOP/s of its three products (P V takes two), where a large product reaches 1119; the matrix
+// pipe is busy 48 % of the time, and a wave reads 32 KB of LDS for each 32 x 64 scores (331 us with P in one operand, at the error
+// told at Wide).  Two waves a SIMD (603 us at one, then) and loads between the barriers, not a tile ahead in
 // registers (which took a fifth more of them for the same time).
 // With few workgroups the tiles are cut into `splits` ranges, which attn_join_kernel joins.
 template <typename T, int DP, int NW>
@@ -672,7 +673,7 @@ __global__ __launch_bounds__(256) void attn_join_rows_kernel(AttnArgs a) {
 // One workgroup = 32 NW queries of one head, keys in tiles of KT: S^T and dP^T = V dO^T share the layout of the forward,
 // dq^T += K^T dS^T.  delta = dout . out is formed here first and left for the dk / dv kernel.  With few workgroups the key tiles
 // are cut into `splits_q` shares, whose fp32 results attn_sum_q_kernel adds in order.  2 x 4001 tokens, 16 on 4 heads of 128,
-// bf16, causal: 399 us, 660 TFLOP/s of its four products (dS K takes two); 350 us with dS in one operand.  The next tile in registers
+// bf16, causal: 394 us, 665 TFLOP/s of its four products (dS K takes two); 350 us with dS in one operand.  The next tile in registers
 // spilled, and took a quarter longer.
 template <typename T, int DP, int NW>
 __global__ __launch_bounds__(NW * 64, sizeof(T) == 2 ? 2 : DP <= 32 ? 3 : DP <= 64 ? 2 : 1) void attn_dq_kernel(AttnArgs a) {
@@ -845,7 +846,7 @@ constexpr bool DKV_V_LDS = sizeof(T) == 2 && DP == 128;
 // One workgroup = 32 NW keys of one key head, one wave = 32 of them; the queries of every head that shares it pass in
 // tiles of 32.  S and dP = dO V^T here have queries as rows: dv^T += dO^T P, dk^T += Q^T dS.  The sums over heads
 // and queries stay in one accumulator in a fixed order: no atomics, the same bits every time.  2 x 4001 tokens, 16 on 4 heads
-// of 128, bf16, causal: 579 us, 680 TFLOP/s of its six products (dO P and Q dS take two); 470 us with P and dS in one operand, 1440 us
+// of 128, bf16, causal: 563 us, 700 TFLOP/s of its six products (dO P and Q dS take two); 461 us with P and dS in one operand, 1440 us
 // without shares and at one wave a SIMD.
 template <typename T, int DP, int NW>
 __global__ __launch_bounds__(NW * 64, sizeof(T) == 2 || DP <= 64 ? 2 : 1) void attn_dkv_kernel(AttnArgs a) {
