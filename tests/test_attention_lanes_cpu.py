@@ -57,7 +57,7 @@ def test_accesses_stay_within_the_tensors(lanes, dtype):
 
 
 @pytest.mark.parametrize("size", [[1, 40, 40, 2, 1, 64], [1, 64, 20, 4, 1, 128], [2, 30, 33, 2, 2, 20], [1, 100, 70, 4, 2, 64],
-                                  [1, 65, 200, 2, 1, 128], [1, 20, 300, 1, 1, 32]])
+                                  [1, 65, 200, 2, 1, 128], [1, 20, 300, 1, 1, 32], [1, 65, 6, 4, 1, 80]])
 def test_large_fp16_gradients(lanes, size):
     """dout of a scaled loss: dout . v far above what fp16 holds, gradients that it holds."""
     run(lanes, [dict(dtype="f16", size=size, v=4.0, dout=1000.0),

@@ -221,7 +221,7 @@ __device__ __forceinline__ float fit_for(float most) {
 }
 // The largest magnitude; zero if that is infinite: such a row's or column's results are lost, and others' scale must not go by it.
 template <typename V>
-__device__ __forceinline__ float most_of(const V& x) {
+__device__ __forceinline__ float most_of(V x) {
   float m = 0.f;
 #pragma unroll
   for (int i = 0; i < (int)(sizeof(V) / sizeof(float)); ++i) m = fmaxf(m, fabsf(x[i]));
@@ -232,9 +232,10 @@ __device__ __forceinline__ float wave_most(float m) {
   for (int o = 32; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
   return __builtin_bit_cast(float, __builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, m)));
 }
-// Makes the values ds of a step fit; acc holds sums of what came before.
+// The values ds of a step, made to fit; acc holds sums of what came before.  (By value: a template's parameter does not keep f32v8's
+// alignment.)
 template <typename V, int N>
-__device__ __forceinline__ void make_fit(V& ds, f32x16 (&acc)[N], float& fit) {
+__device__ __forceinline__ V make_fit(V ds, f32x16 (&acc)[N], float& fit) {
   const float most = most_of(ds);
   if (__any(most * fit > FIT_LIMIT)) {
     const float now = fit_for(wave_most(most));
@@ -248,6 +249,7 @@ __device__ __forceinline__ void make_fit(V& ds, f32x16 (&acc)[N], float& fit) {
 #pragma unroll
     for (int i = 0; i < (int)(sizeof(V) / sizeof(float)); ++i) ds[i] *= fit;
   }
+  return ds;
 }
 
 // One bit per key of the tile at key0: below the sequence's length and not masked.  The same in every wave.
@@ -783,7 +785,7 @@ __global__ __launch_bounds__(NW * 64, sizeof(T) == 2 ? 2 : DP <= 32 ? 3 : DP <= 
         for (int r = 0; r < 16; ++r)
           if (t * 32 + 8 * (r / 4) + r % 4 > room) s[r] = 0.f;
       }
-      if (FIT<T>) make_fit(s, acc, fit);
+      if (FIT<T>) s = make_fit(s, acc, fit);
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
         const Wide<T> ds(part8(s, c));
@@ -983,7 +985,7 @@ __global__ __launch_bounds__(NW * 64, sizeof(T) == 2 || DP <= 64 ? 2 : 1) void a
       }
       const Wide<T> p(p8);
       p.mma_all(dv, [&](int dt) { return frag_at<T>(gx, TileX<T, QT>::frag(dt * 32 + col, c, half)); });
-      if (FIT<T>) make_fit(ds8, dk, fit);
+      if (FIT<T>) ds8 = make_fit(ds8, dk, fit);
       const Wide<T> ds(ds8);
       ds.mma_all(dk, [&](int dt) { return frag_at<T>(qx, TileX<T, QT>::frag(dt * 32 + col, c, half)); });
     }
